@@ -11,7 +11,10 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libgan_amd.so"
 SOURCES = ["capi.hip", "conv_direct.hip", "conv_mfma.hip", "conv_gemm.hip", "conv_pp.hip", "conv_win.hip", "conv_stream.hip", "conv_swin.hip", "resunit.hip", "conv_coop.hip", "wgrad_mfma.hip", "wgrad_gemm.hip", "wgrad_cin1_mfma.hip", "thin.hip", "lstm.hip", "lstm_persist.hip", "elementwise.hip", "cnorm.hip", "stft.hip"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their forms give wrong results now and then on these cards (the host pass warns
+# that it does not know the feature: harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(out: Path, deps) -> bool:
