@@ -99,6 +99,66 @@ class LstmBwdParams(C.Structure):
                [(n, C.c_int) for n in ("B", "T", "H", "act_dtype", "w_dtype")] + [("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+class CausalConvParams(C.Structure):
+    """ga_causal_conv_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "state", "lengths", "y", "last")] + \
+               [(n, C.c_long) for n in ("x_bs", "x_ts")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "K", "act")]
+
+
+class CausalConvBwdParams(C.Structure):
+    """ga_causal_conv_bwd_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "state", "lengths", "dy", "dlast", "dx", "dstate", "dw", "dbias", "ws")] + \
+               [(n, C.c_long) for n in ("x_bs", "x_ts")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "K", "act")]
+
+
+class CausalConvStepParams(C.Structure):
+    """ga_causal_conv_step_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "state", "y")] + \
+               [(n, C.c_long) for n in ("x_bs", "state_bs")] + \
+               [(n, C.c_int) for n in ("B", "C", "K", "act")]
+
+
+class ScanBuffers(C.Structure):
+    """ga_scan_buffers (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_size_t) for n in ("maps", "hs", "ends", "ends_step", "dmaps", "dparams")]
+
+
+class ScanParams(C.Structure):
+    """ga_scan_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "z", "Bm", "Cm", "A", "D", "delta_bias", "state", "lengths", "y", "last", "maps", "hs", "ends", "ends_step")] + \
+               [(n, C.c_long) for n in ("u_bs", "u_ts", "delta_bs", "delta_ts", "z_bs", "z_ts", "b_bs", "b_ts", "c_bs", "c_ts")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "N", "G", "softplus")]
+
+
+class ScanBwdParams(C.Structure):
+    """ga_scan_bwd_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "z", "A", "D", "delta_bias", "lengths", "dy", "dlast", "maps", "hs", "du", "ddelta", "dz", "dBm", "dCm", "dA", "dD", "ddelta_bias", "dstate", "ends", "ends_step", "dmaps", "dparams")] + \
+               [(n, C.c_long) for n in ("u_bs", "u_ts", "delta_bs", "delta_ts", "z_bs", "z_ts")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "N", "G", "softplus")]
+
+
+class ScanStepParams(C.Structure):
+    """ga_scan_step_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "z", "Bm", "Cm", "A", "D", "delta_bias", "state", "y")] + \
+               [(n, C.c_long) for n in ("u_bs", "delta_bs", "z_bs", "b_bs", "c_bs", "state_bs")] + \
+               [(n, C.c_int) for n in ("B", "C", "N", "G", "softplus")]
+
+
+class BlockNormParams(C.Structure):
+    """ga_block_norm_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "branch", "gate", "w", "b", "wp", "bp", "scale", "ab", "r", "y", "stats")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "post", "layer", "gate_rows")] + \
+               [(n, C.c_float) for n in ("eps",)]
+
+
+class BlockNormBwdParams(C.Structure):
+    """ga_block_norm_bwd_params (include/gan_amd.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "branch", "gate", "w", "b", "wp", "bp", "scale", "ab", "stats", "dr", "dy", "dx", "dbranch", "dgate", "dw", "db", "dwp", "dbp", "dscale", "dab", "ws")] + \
+               [(n, C.c_int) for n in ("B", "T", "C", "post", "layer", "gate_rows")]
+
+
 _P, _I, _F, _Z = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 _SIGNATURES = {
     "ga_conv": [C.POINTER(ConvParams), _I, _I, _P],
@@ -156,6 +216,17 @@ _SIGNATURES = {
     "ga_stft_unpad_bwd": [_P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "ga_lstm_fwd": [C.POINTER(LstmParams), _P],
     "ga_lstm_bwd": [C.POINTER(LstmBwdParams), _P],
+    "ga_causal_conv_fwd": [C.POINTER(CausalConvParams), _I, _P],
+    "ga_causal_conv_bwd": [C.POINTER(CausalConvBwdParams), _I, _P],
+    "ga_causal_conv_step": [C.POINTER(CausalConvStepParams), _I, _P],
+    "ga_causal_conv_bwd_ws_elems": [_I, _I, _I, _I],
+    "ga_scan_sizes": [_I, _I, _I, _I, _I, C.POINTER(ScanBuffers)],
+    "ga_scan_fwd": [C.POINTER(ScanParams), _I, _P],
+    "ga_scan_bwd": [C.POINTER(ScanBwdParams), _I, _P],
+    "ga_scan_step": [C.POINTER(ScanStepParams), _I, _P],
+    "ga_block_norm_fwd": [C.POINTER(BlockNormParams), _I, _I, _P],
+    "ga_block_norm_bwd": [C.POINTER(BlockNormBwdParams), _I, _I, _P],
+    "ga_block_norm_bwd_ws_elems": [_I, _I, _I, _I],
     "ga_grad_sqnorm": [_P, _Z, _P, _P],
     "ga_adamw_fused": [_P, _P, _P, _P, _Z, _F, _F, _F, _F, _F, _I, _F, _F, _P, _I, _P],
     "ga_adamw_fused_devstep": [_P, _P, _P, _P, _Z, _F, _F, _F, _F, _F, _P, _F, _F, _P, _I, _P],
@@ -181,7 +252,8 @@ def lib():
             fn.restype = C.c_int
         l.ga_packed_elems.argtypes = [_I, _I, _I, _I, _I]
         l.ga_packed_elems.restype = C.c_size_t
-        l.ga_wgrad_workspace_elems.restype = C.c_size_t
+        for name in ("ga_wgrad_workspace_elems", "ga_causal_conv_bwd_ws_elems", "ga_block_norm_bwd_ws_elems"):
+            getattr(l, name).restype = C.c_size_t
         l.ga_lstm_persist_workspace_bytes.argtypes = [_I]
         l.ga_lstm_persist_workspace_bytes.restype = C.c_size_t
         l.ga_build_target.argtypes = []
@@ -194,6 +266,7 @@ _ERR = {1: "GA_ERR_ARG (bad shape / unsupported configuration)", 2: "GA_ERR_LAUN
         3: "GA_ERR_ALIGN (pointer alignment)", 4: "GA_ERR_UNSUPPORTED (this variant does not take the shape)",
         5: "GA_ERR_SCRATCH (problem larger than the library's fixed split-K scratch: use ga_conv with a workspace)"}
 SPLITK_STATIC_FLOATS = 8 << 20
+CCONV_MAX_TAPS, SCAN_MAX_STATES, BNORM_MAX_C = 8, 64, 8192
 
 
 def check(rc: int, what: str) -> None:

@@ -10,7 +10,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libgan_amd.so"
-SOURCES = ["capi.hip", "conv_direct.hip", "conv_mfma.hip", "conv_gemm.hip", "conv_pp.hip", "conv_win.hip", "conv_stream.hip", "conv_swin.hip", "resunit.hip", "conv_coop.hip", "wgrad_mfma.hip", "wgrad_gemm.hip", "wgrad_cin1_mfma.hip", "thin.hip", "lstm.hip", "lstm_persist.hip", "elementwise.hip", "cnorm.hip", "stft.hip"]
+SOURCES = ["capi.hip", "conv_direct.hip", "conv_mfma.hip", "conv_gemm.hip", "conv_pp.hip", "conv_win.hip", "conv_stream.hip", "conv_swin.hip", "resunit.hip", "conv_coop.hip", "wgrad_mfma.hip", "wgrad_gemm.hip", "wgrad_cin1_mfma.hip", "thin.hip", "lstm.hip", "lstm_persist.hip", "elementwise.hip", "cnorm.hip", "stft.hip", "causal_conv.hip", "scan.hip", "block_norm.hip"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their forms give wrong results now and then on these cards (the host pass warns
 # that it does not know the feature: harmless)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
@@ -26,7 +26,7 @@ def _stale(out: Path, deps) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [CSRC / "common.h", CSRC / "swin_common.h", HERE.parent / "include" / "gan_amd.h"]
+    headers = [CSRC / "common.h", CSRC / "swin_common.h", CSRC / "seq_common.h", HERE.parent / "include" / "gan_amd.h"]
     objdir = CSRC / "build"
     objdir.mkdir(exist_ok=True)
     jobs = []

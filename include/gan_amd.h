@@ -519,6 +519,114 @@ typedef struct ga_lstm_bwd_params {
 } ga_lstm_bwd_params;
 int ga_lstm_bwd(const ga_lstm_bwd_params* h_params, ga_stream_t stream);
 
+/* ---- sequence operators: linear-time mixing along time for models on codec latents, next to ga_conv / ga_lstm_* / ga_gn_* ----
+ * No reference call site: they extend the operator set.  Element strides (*_bs batch, *_ts time) let an input be a channel slice of a wider
+ * projection; outputs are packed.  lengths (int32 [B] or NULL): item b ends at row lengths[b] (clamped to 0 .. T); rows behind it are neither
+ * read nor counted, their outputs and gradients are zero.  No atomics: results do not depend on timing.  Buffers that the caller sizes with a
+ * ga_*_sizes / ga_*_elems call need no initialisation. */
+
+/* Short causal depthwise convolution:  y[b][t][c] = act(bias[c] + sum_k w[c][k] x[b][t-(K-1)+k][c]), act GA_ACT_NONE or GA_ACT_SILU.
+ * Rows before 0 come from state [B][K-1][C] (NULL: zero); last [B][K-1][C] (may be NULL) receives the K-1 rows that end the sequence. */
+#define GA_CCONV_MAX_TAPS 8
+typedef struct ga_causal_conv_params {
+    const void* x; const float* w; const float* bias; const void* state; const int* lengths;
+    void* y; void* last;
+    long x_bs, x_ts;
+    int B, T, C, K, act;
+} ga_causal_conv_params;
+int ga_causal_conv_fwd(const ga_causal_conv_params* h_params, int dtype, ga_stream_t stream);
+/* dy [B][T][C], dlast [B][K-1][C] or NULL -> dx [B][T][C], dstate [B][K-1][C] or NULL, dw [C][K], dbias [C] or NULL; ws: fp32,
+ * ga_causal_conv_bwd_ws_elems() (0: sizes out of range) */
+typedef struct ga_causal_conv_bwd_params {
+    const void* x; const float* w; const float* bias; const void* state; const int* lengths;
+    const void* dy; const void* dlast;
+    void* dx; void* dstate; float* dw; float* dbias; float* ws;
+    long x_bs, x_ts;
+    int B, T, C, K, act;
+} ga_causal_conv_bwd_params;
+size_t ga_causal_conv_bwd_ws_elems(int B, int T, int C, int K);
+int ga_causal_conv_bwd(const ga_causal_conv_bwd_params* h_params, int dtype, ga_stream_t stream);
+/* one token: x [B][C] (row stride x_bs), y [B][C]; state [B][K-1][C] (items state_bs apart) moves on by a row in place */
+typedef struct ga_causal_conv_step_params {
+    const void* x; const float* w; const float* bias; void* state; void* y;
+    long x_bs, state_bs;
+    int B, C, K, act;
+} ga_causal_conv_step_params;
+int ga_causal_conv_step(const ga_causal_conv_step_params* h_params, int dtype, ga_stream_t stream);
+
+/* Selective state space scan over h [C][N] per item (fp32):  D_t = softplus(delta_t + delta_bias) (or the sum itself when softplus = 0),
+ *   h_t = exp(D_t A) h_{t-1} + D_t u_t B_t,   y_t = (sum_n C_t[n] h_t[n] + D u_t) silu(z_t)
+ * u, delta, z (NULL: no gate) [B][T][C]; Bm, Cm [B][T][G][N] with [G][N] packed, channel c reads group c / (C / G); A [C][N], D, delta_bias [C]
+ * fp32 (the last two may be NULL); state [B][C][N] fp32 (NULL: zero); last [B][C][N] (may be NULL) receives the state at the item's end.
+ * maps / hs / ends / ends_step: fp32 buffers of ga_scan_sizes() elements; maps and hs are what the backward pass reads (hs NULL: not wanted). */
+#define GA_SCAN_MAX_STATES 64
+typedef struct ga_scan_buffers {
+    size_t maps;      /* B and C in float32, in the kernels' order */
+    size_t hs;        /* the state at every 16th row */
+    size_t ends;      /* per chunk of a sequence that is worked on in parallel: its own end state (forward) / start adjoint (backward) */
+    size_t ends_step; /* and the sum of its steps; both 0 when one chunk does */
+    size_t dmaps;     /* backward: the gradients of B and C per block of channels */
+    size_t dparams;   /* backward: the gradients of A, D and delta_bias per chunk */
+} ga_scan_buffers;
+int ga_scan_sizes(int B, int T, int C, int N, int G, ga_scan_buffers* h_out);
+typedef struct ga_scan_params {
+    const void* u; const void* delta; const void* z; const void* Bm; const void* Cm;
+    const float* A; const float* D; const float* delta_bias; const float* state; const int* lengths;
+    void* y; float* last;
+    float* maps; float* hs; float* ends; float* ends_step;
+    long u_bs, u_ts, delta_bs, delta_ts, z_bs, z_ts, b_bs, b_ts, c_bs, c_ts;
+    int B, T, C, N, G, softplus;
+} ga_scan_params;
+int ga_scan_fwd(const ga_scan_params* h_params, int dtype, ga_stream_t stream);
+/* dy [B][T][C], dlast [B][C][N] or NULL, maps and hs as the forward call left them -> du, ddelta, dz (NULL iff z is) [B][T][C], dBm, dCm
+ * [B][T][G][N], dA [C][N], dD, ddelta_bias [C] or NULL, dstate [B][C][N] or NULL */
+typedef struct ga_scan_bwd_params {
+    const void* u; const void* delta; const void* z;
+    const float* A; const float* D; const float* delta_bias; const int* lengths;
+    const void* dy; const float* dlast; const float* maps; const float* hs;
+    void* du; void* ddelta; void* dz; void* dBm; void* dCm;
+    float* dA; float* dD; float* ddelta_bias; float* dstate;
+    float* ends; float* ends_step; float* dmaps; float* dparams;
+    long u_bs, u_ts, delta_bs, delta_ts, z_bs, z_ts;
+    int B, T, C, N, G, softplus;
+} ga_scan_bwd_params;
+int ga_scan_bwd(const ga_scan_bwd_params* h_params, int dtype, ga_stream_t stream);
+/* one token: u, delta, z [B][C] and Bm, Cm [B][G][N] (rows *_bs apart), y [B][C]; state [B][C][N] (items state_bs apart) is updated in place */
+typedef struct ga_scan_step_params {
+    const void* u; const void* delta; const void* z; const void* Bm; const void* Cm;
+    const float* A; const float* D; const float* delta_bias;
+    float* state; void* y;
+    long u_bs, delta_bs, z_bs, b_bs, c_bs, state_bs;
+    int B, C, N, G, softplus;
+} ga_scan_step_params;
+int ga_scan_step(const ga_scan_step_params* h_params, int dtype, ga_stream_t stream);
+
+/* The edges of a residual block, rows of C <= GA_BNORM_MAX_C:  n = norm(branch) wp + bp when post, else branch;  r = x + scale gate n;
+ * y = (norm(r) w + b)(1 + a) + s.  norm: v / sqrt(mean(v^2) + eps), or with layer = 1 (v - mean) / sqrt(var + eps).  x, r in xdtype; branch, y
+ * and a gate per row in dtype (xdtype = dtype, or fp32 with bf16).  w, b, wp, bp, scale [C] fp32, each may be NULL (1, 0, 1, 0, 1);
+ * gate: NULL, fp32 [B][C] (gate_rows = 0) or dtype [B][T][C] (gate_rows = 1); ab: NULL or fp32 [B][2C] = (a | s).  branch NULL: r is x, not
+ * written.  stats [B*T][4] fp32 or NULL: means and reciprocal deviations of the two norms for the backward pass. */
+#define GA_BNORM_MAX_C 8192
+typedef struct ga_block_norm_params {
+    const void* x; const void* branch; const void* gate;
+    const float* w; const float* b; const float* wp; const float* bp; const float* scale; const float* ab;
+    void* r; void* y; float* stats;
+    int B, T, C, post, layer, gate_rows;
+    float eps;
+} ga_block_norm_params;
+int ga_block_norm_fwd(const ga_block_norm_params* h_params, int xdtype, int dtype, ga_stream_t stream);
+/* dr (xdtype) and / or dy (dtype) -> dx (xdtype), dbranch, dgate (like gate), dab, dw, db, dwp, dbp, dscale (fp32, each may be NULL); ws: fp32,
+ * ga_block_norm_bwd_ws_elems(..., by_item = there is an ab or a gate per item) */
+typedef struct ga_block_norm_bwd_params {
+    const void* x; const void* branch; const void* gate;
+    const float* w; const float* b; const float* wp; const float* bp; const float* scale; const float* ab;
+    const float* stats; const void* dr; const void* dy;
+    void* dx; void* dbranch; void* dgate; float* dw; float* db; float* dwp; float* dbp; float* dscale; float* dab; float* ws;
+    int B, T, C, post, layer, gate_rows;
+} ga_block_norm_bwd_params;
+size_t ga_block_norm_bwd_ws_elems(int B, int T, int C, int by_item);
+int ga_block_norm_bwd(const ga_block_norm_bwd_params* h_params, int xdtype, int dtype, ga_stream_t stream);
+
 /* library identification: returns the gfx target the code objects were built for ("gfx950") */
 const char* ga_build_target(void);
 
