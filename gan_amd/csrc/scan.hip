@@ -6,6 +6,7 @@
 // a wave, and passes through LDS; B and C, which all channels of a group share, are first laid out in float32 in the order in which
 // the waves read them (scan_maps_kernel) and come in as scalar loads, so that they cost no vector instruction and no LDS bandwidth.
 #include "seq_common.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -16,24 +17,23 @@ constexpr int MAX_CHUNKS = 64;  // a block adds up the chunks before (behind) it
 typedef const __attribute__((address_space(4))) float* uniform_ptr;
 
 struct Plan {
-    int NB, SB, NP;           // states per wave and state block, state blocks, 4 * NB * SB
+    int NS, NP;               // states of a wave, of the four waves
     int Cg, cbg, nCb;         // channels of a group, 64-channel blocks of a group, of all groups
-    int Tp, tiles;            // rows rounded up to a tile
+    int tiles;                // of a sequence
     int chunks, chunk_tiles;  // tiles of a chunk
 };
 
 Plan make_plan(int B, int T, int C, int N, int G) {
     Plan q;
-    q.NB = N <= 4 ? 1 : N <= 8 ? 2 : 4;
-    q.SB = N <= 16 ? 1 : N <= 32 ? 2 : 4;
-    q.NP = 4 * q.NB * q.SB;
+    q.NS = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
+    q.NP = 4 * q.NS;
     q.Cg = C / G;
     q.cbg = (q.Cg + 63) / 64;
     q.nCb = q.cbg * G;
     q.tiles = (T + TS - 1) / TS;
-    q.Tp = q.tiles * TS;
     const long blocks = (long)B * q.nCb;
-    long want = (1024 + blocks - 1) / blocks;
+    static const long target = getenv("SCAN_BLOCKS") ? atol(getenv("SCAN_BLOCKS")) : 1024;
+    long want = (target + blocks - 1) / blocks;
     if (want > MAX_CHUNKS) want = MAX_CHUNKS;
     if (want > q.tiles) want = q.tiles;
     if (want < 1) want = 1;
@@ -51,367 +51,472 @@ struct BwdArgs {
     Plan q;
 };
 
-// state index of (wave, state block, j)
-__device__ __forceinline__ int state_of(int w, int sb, int j, int NB) { return sb * 4 * NB + w * NB + j; }
-
-// maps[b][row][group][wave][sb][B: NB | C: NB] in float32; zero rows behind an item's length and up to the whole tile, zero states behind N
+// maps[b][group][tile][wave][row][B: NS | C: NS] in float32, wave w holding the states w NS .. w NS + NS - 1; zero rows behind an item's length and
+// up to the whole tile, zero states behind N
 template <typename T>
 __global__ __launch_bounds__(256) void scan_maps_kernel(const T* __restrict__ Bm, const T* __restrict__ Cm, float* __restrict__ maps,
                                                         const int* __restrict__ lengths, Plan q, int B, int Tn, int N, int G, long b_bs,
                                                         long b_ts, long c_bs, long c_ts) {
-    const size_t total = (size_t)B * q.Tp * G * q.NP;
+    const size_t total = (size_t)B * G * q.tiles * TS * q.NP;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-        const int s = (int)(i % q.NP);
-        const size_t row = i / q.NP;
-        const int g = (int)(row % G);
-        const size_t bt = row / G;
-        const int t = (int)(bt % q.Tp), b = (int)(bt / q.Tp);
-        const int w = s / (q.NB * q.SB), sb = (s / q.NB) % q.SB, j = s % q.NB;
-        const int n = sb * 4 * q.NB + w * q.NB + j;
+        const int j = (int)(i % q.NS);
+        const size_t row = i / q.NS;  // of a wave
+        const int r = (int)(row % TS), w = (int)(row / TS % 4);
+        const size_t bgt = row / (4 * TS);
+        const int t = (int)(bgt % q.tiles) * TS + r, g = (int)(bgt / q.tiles % G), b = (int)(bgt / q.tiles / G), n = w * q.NS + j;
         const bool live = n < N && t < sq_len(lengths, b, Tn);
         const float vb = live ? (float)Bm[(size_t)b * b_bs + (size_t)t * b_ts + (size_t)g * N + n] : 0.f;
         const float vc = live ? (float)Cm[(size_t)b * c_bs + (size_t)t * c_ts + (size_t)g * N + n] : 0.f;
-        float* o = maps + row * (2 * q.NP) + (size_t)(w * q.SB + sb) * 2 * q.NB + j;
-        o[0] = vb;
-        o[q.NB] = vc;
+        maps[row * 2 * q.NS + j] = vb;
+        maps[row * 2 * q.NS + q.NS + j] = vc;
+    }
+}
+
+// where a block and a lane are
+struct Place {
+    int lane, w, chunk, b, g, d, len, tile0, tile1;
+    bool ok;
+    size_t item;  // first tile of the item's group in the maps
+};
+__device__ __forceinline__ Place place(const Plan& q, int nch, int first_chunk, int G, int T, const int* lengths) {
+    Place x;
+    x.lane = threadIdx.x & 63;
+    x.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cb = blockIdx.x % q.nCb, rest = blockIdx.x / q.nCb;
+    x.chunk = first_chunk + rest % nch;
+    x.b = rest / nch;
+    x.g = cb / q.cbg;
+    const int din = (cb % q.cbg) * 64 + x.lane;
+    x.ok = din < q.Cg;
+    x.d = x.g * q.Cg + (x.ok ? din : q.Cg - 1);
+    x.len = sq_len(lengths, x.b, T);
+    x.tile0 = x.chunk * q.chunk_tiles;
+    x.tile1 = min(x.tile0 + q.chunk_tiles, q.tiles);
+    x.item = (size_t)(x.b * G + x.g) * q.tiles;
+    return x;
+}
+
+// carry[s] <- exp(A sum of steps) carry[s] + end state, over the chunks from, from + dir, ... (count of them), eight loads in flight
+template <int NS>
+__device__ __forceinline__ void chain(float (&carry)[NS], const float (&A2)[NS], const float* ends, const float* ends_step, const Plan& q, int C, int b,
+                                      int w, int d, int from, int dir, int count) {
+    constexpr int U = NS <= 4 ? 8 : NS <= 8 ? 4 : 2;
+    for (int k = 0; k < count; k += U) {
+        float sum[U], end[U][NS];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const size_t e = (size_t)b * q.chunks + (from + dir * min(k + i, count - 1));
+            sum[i] = ends_step[e * C + d];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) end[i][s] = ends[(e * q.NP + w * NS + s) * C + d];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (k + i < count) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s) carry[s] = fmaf(__builtin_amdgcn_exp2f(sum[i] * A2[s]), carry[s], end[i][s]);
+            }
     }
 }
 
 // ENDS: only the state that each chunk but the last leaves behind when it starts from zero, and the sum of its steps
 // (the chunk's decay is exp(A * that sum)).  Otherwise the outputs, each chunk from the states of the chunks before it.
-template <typename T, int NB, int SB, bool ENDS>
+template <typename T, int NS, bool ENDS>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     const ga_scan_params& p = a.p;
     const Plan& q = a.q;
-    constexpr int NS = NB * SB;
+    // rows whose B and C are in scalar registers at a time, twice (one set on its way)
+    constexpr int U = ENDS ? (NS <= 4 ? 4 : NS <= 8 ? 2 : 1) : (NS <= 4 ? 2 : 1);
     __shared__ float2 sd[TS][64];
     __shared__ float sy[ENDS ? 1 : 4][ENDS ? 1 : TS][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cb = blockIdx.x % q.nCb, rest = blockIdx.x / q.nCb;
-    const int nch = ENDS ? q.chunks - 1 : q.chunks;
-    const int chunk = rest % nch, b = rest / nch;
-    const int g = cb / q.cbg, din = (cb % q.cbg) * 64 + lane;
-    const bool ok = din < q.Cg;
-    const int d = g * q.Cg + (ok ? din : q.Cg - 1);
-    const int len = sq_len(p.lengths, b, p.T);
+    const Place x = place(q, ENDS ? q.chunks - 1 : q.chunks, 0, p.G, p.T, p.lengths);
+    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
     float A2[NS], h[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int n = state_of(w, s / NB, s % NB, NB);
+        const int n = w * NS + s;
         A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
         h[s] = 0.f;
-        if (!ENDS && p.state && n < p.N) h[s] = p.state[((size_t)b * p.C + d) * p.N + n];
+        if (!ENDS && p.state && n < p.N) h[s] = p.state[((size_t)x.b * p.C + d) * p.N + n];
     }
-    if (!ENDS) {
-        for (int k = 0; k < chunk; ++k) {
-            const size_t e = (size_t)b * q.chunks + k;
-            const float sum = p.ends_step[e * p.C + d];
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int n = state_of(w, s / NB, s % NB, NB);
-                h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), h[s], p.ends[(e * q.NP + n) * p.C + d]);
-            }
-        }
-    }
-    const T* up = (const T*)p.u + (size_t)b * p.u_bs + d;
-    const T* dp = (const T*)p.delta + (size_t)b * p.delta_bs + d;
-    const T* zp = p.z ? (const T*)p.z + (size_t)b * p.z_bs + d : nullptr;
-    T* yp = ENDS ? nullptr : (T*)p.y + (size_t)b * p.T * p.C + d;
-    const int tile0 = chunk * q.chunk_tiles, tile1 = min(tile0 + q.chunk_tiles, q.tiles);
-    const size_t mrow = (size_t)p.G * 2 * q.NP;
-    uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((size_t)b * q.Tp + (size_t)tile0 * TS) * mrow + (size_t)g * 2 * q.NP + (size_t)w * SB * 2 * NB);
-    float ru[RPW], rd[RPW], rz[RPW], total = 0.f;
-    auto load = [&](int tile) __attribute__((always_inline)) {
+    const T* up = (const T*)p.u + (size_t)x.b * p.u_bs;
+    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
+    const T* zp = ENDS || !p.z ? nullptr : (const T*)p.z + (size_t)x.b * p.z_bs;
+    T ru[RPW], rd[RPW], rz[RPW];
+    float total = 0.f;
+    auto load = [&](int tile) __attribute__((always_inline)) {  // (rows behind the last one read that one: no branch between the loads)
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            const int t = tile * TS + w * RPW + r;
-            const bool live = ok && t < len;
-            ru[r] = live ? (float)up[(size_t)t * p.u_ts] : 0.f;
-            rd[r] = live ? (float)dp[(size_t)t * p.delta_ts] : 0.f;
-            rz[r] = !ENDS && zp && live ? (float)zp[(size_t)t * p.z_ts] : 0.f;
+            const int t = min(tile * TS + w * RPW + r, p.T - 1);
+            ru[r] = (up + (size_t)t * p.u_ts)[d];
+            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
+            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
         }
     };
-    load(tile0);
-    for (int tile = tile0; tile < tile1; ++tile) {
+    load(x.tile0);
+    if (!ENDS) chain<NS>(h, A2, p.ends, p.ends_step, q, p.C, x.b, w, d, 0, 1, x.chunk);
+    uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + x.tile0) * 4 + w) * (TS * 2 * NS));
+    float m[2][U][2 * NS];
+    auto fetch = [&](float (&o)[U][2 * NS], uniform_ptr from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int j = 0; j < (ENDS ? NS : 2 * NS); ++j) o[i][j] = from[i * 2 * NS + j];
+    };
+    for (int tile = x.tile0; tile < x.tile1; ++tile) {
         float cu[RPW], cz[RPW];
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
-            const float raw = rd[r] + bias;
-            float step = p.softplus ? sq_softplus(raw) : raw;
-            step = ok && t < len ? step : 0.f;
-            cu[r] = ru[r];
-            cz[r] = rz[r];
+            const bool live = x.ok && t < len;
+            const float raw = (float)rd[r] + bias;
+            const float step = live ? p.softplus ? sq_softplus(raw) : raw : 0.f;
+            cu[r] = live ? (float)ru[r] : 0.f;
+            cz[r] = zp ? (float)rz[r] : 0.f;
             total += step;
-            sd[row][lane] = make_float2(step, step * ru[r]);
+            sd[row][lane] = make_float2(step, step * cu[r]);
         }
+        fetch(m[0], mp);
         __syncthreads();
-        if (tile + 1 < tile1) load(tile + 1);
-        if (!ENDS && p.hs && ok) {
+        if (tile + 1 < x.tile1) load(tile + 1);
+        if (!ENDS && p.hs && x.ok) {
+            float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS) * p.C;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int n = state_of(w, s / NB, s % NB, NB);
-                if (n < p.N) p.hs[(((size_t)b * q.tiles + tile) * p.N + n) * p.C + d] = h[s];
-            }
+            for (int s = 0; s < NS; ++s) (hp + (size_t)s * p.C)[d] = h[s];
         }
+        float2 v[2][U];
+        float y[TS];
 #pragma unroll
-        for (int t = 0; t < TS; ++t) {
-            const float2 v = sd[t][lane];
-            float y = 0.f;
+        for (int i = 0; i < U; ++i) v[0][i] = sd[i][lane];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const float bv = mp[t * mrow + (s / NB) * 2 * NB + s % NB];
-                h[s] = fmaf(__builtin_amdgcn_exp2f(v.x * A2[s]), h[s], v.y * bv);
-                if (!ENDS) y = fmaf(mp[t * mrow + (s / NB) * 2 * NB + NB + s % NB], h[s], y);
+        for (int k = 0; k < TS / U; ++k) {
+            if (k + 1 < TS / U) {
+                fetch(m[(k + 1) & 1], mp + (k + 1) * U * 2 * NS);
+#pragma unroll
+                for (int i = 0; i < U; ++i) v[(k + 1) & 1][i] = sd[(k + 1) * U + i][lane];
             }
-            if (!ENDS) sy[w][t][lane] = y;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const float2 c = v[k & 1][i];
+                const float* mm = m[k & 1][i];
+                float o = 0.f;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    h[s] = fmaf(__builtin_amdgcn_exp2f(c.x * A2[s]), h[s], c.y * mm[s]);
+                    if (!ENDS) o = fmaf(mm[NS + s], h[s], o);
+                }
+                y[k * U + i] = o;
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        mp += TS * mrow;
+        mp += 4 * TS * 2 * NS;
+        if (!ENDS) {
+#pragma unroll
+            for (int t = 0; t < TS; ++t) sy[w][t][lane] = y[t];
+        }
         __syncthreads();
         if (!ENDS) {
 #pragma unroll
             for (int r = 0; r < RPW; ++r) {
                 const int row = w * RPW + r, t = tile * TS + row;
-                float y = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                if (zp) y *= sq_silu(cz[r]);
-                if (ok && t < p.T) yp[(size_t)t * p.C] = (T)(t < len ? y : 0.f);
+                float o = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
+                if (zp) o *= sq_silu(cz[r]);
+                if (x.ok && t < p.T) ((T*)p.y + ((size_t)x.b * p.T + t) * p.C)[d] = (T)(t < len ? o : 0.f);
             }
         }
     }
     if (ENDS) {
-        const size_t e = (size_t)b * q.chunks + chunk;
-        if (ok) {
+        const size_t e = (size_t)x.b * q.chunks + x.chunk;
+        if (x.ok) {
 #pragma unroll
-            for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + state_of(w, s / NB, s % NB, NB)) * p.C + d] = h[s];
+            for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + w * NS + s) * p.C + d] = h[s];
         }
         sd[w][lane].x = total;
         __syncthreads();
-        if (w == 0 && ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
-    } else if (p.last && chunk == q.chunks - 1 && ok) {
+        if (w == 0 && x.ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
+    } else if (p.last && x.chunk == q.chunks - 1 && x.ok) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int n = state_of(w, s / NB, s % NB, NB);
-            if (n < p.N) p.last[((size_t)b * p.C + d) * p.N + n] = h[s];
+            const int n = w * NS + s;
+            if (n < p.N) p.last[((size_t)x.b * p.C + d) * p.N + n] = h[s];
         }
     }
 }
 
-// Sum of each of V values over the 64 lanes; lane l leaves with the sum of value (the top log2 V bits of l).  Each step sends one half of the
-// values each way across a lane bit, so that the work halves with it: 2V - 2 adds and exchanges in place of 6V.
+// Sums over the 64 lanes of many values at once: each step sends one half of the values each way across a lane bit, so that the work halves
+// with it (V values cost 2V - 2 exchanges and adds and not 6V).  permlane swaps for the upper two lane bits, DPP for the others.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
+__device__ __forceinline__ float fold32(float a, float b) {  // lanes 0-31: a over both halves, 32-63: b
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float fold(float a, float b, bool up) {
+    return (up ? b : a) + dpp<CTRL>(up ? a : b);
+}
+// n values (a power of two) in v; lane l leaves with v[0] = the sum of value (the top log2 n bits of l)
 template <int V>
 __device__ __forceinline__ float lane_sums(float (&v)[V], int lane) {
-    static_assert(V >= 2 && V <= 64 && (V & (V - 1)) == 0, "a power of two");
+    static_assert(V >= 1 && V <= 64 && (V & (V - 1)) == 0, "a power of two");
     int n = V;
-#define SQ_SWAP(BUILTIN)                                                                                            \
-    if (n > 1) {                                                                                                    \
-        n >>= 1;                                                                                                    \
-        _Pragma("unroll") for (int i = 0; i < n; ++i) {                                                             \
-            const auto x = BUILTIN(__float_as_uint(v[i]), __float_as_uint(v[i + n]), false, false);                 \
-            v[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);                                                   \
-        }                                                                                                           \
-    } else {                                                                                                        \
-        const auto x = BUILTIN(__float_as_uint(v[0]), __float_as_uint(v[0]), false, false);                         \
-        v[0] = __uint_as_float(x[0]) + __uint_as_float(x[1]);                                                       \
-    }
-#define SQ_STEP(BIT, CTRL)                                                                                          \
-    if (n > 1) {                                                                                                    \
-        n >>= 1;                                                                                                    \
-        const bool up = lane & BIT;                                                                                 \
-        _Pragma("unroll") for (int i = 0; i < n; ++i) {                                                             \
-            const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];                                   \
-            v[i] = keep + dpp<CTRL>(give);                                                                          \
-        }                                                                                                           \
-    } else                                                                                                          \
-        v[0] += dpp<CTRL>(v[0]);
-    SQ_SWAP(__builtin_amdgcn_permlane32_swap)
-    SQ_SWAP(__builtin_amdgcn_permlane16_swap)
-    SQ_STEP(8, 0x128)  // rotate by 8 within 16
-    SQ_STEP(4, 0x141)  // mirror within 8
-    SQ_STEP(2, 0x4E)   // quads: 2 3 0 1
-    SQ_STEP(1, 0xB1)   // quads: 1 0 3 2
-#undef SQ_SWAP
-#undef SQ_STEP
+#define SQ_FOLD(FN, ...)                                                              \
+    if (n > 1) {                                                                      \
+        n >>= 1;                                                                      \
+        _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = FN(v[i], v[i + n] __VA_ARGS__); \
+    } else
+    SQ_FOLD(fold32) v[0] = fold32(v[0], v[0]);
+    SQ_FOLD(fold16) v[0] = fold16(v[0], v[0]);
+    SQ_FOLD(fold<0x128>, , lane & 8) v[0] += dpp<0x128>(v[0]);  // rotate by 8 within 16
+    SQ_FOLD(fold<0x141>, , lane & 4) v[0] += dpp<0x141>(v[0]);  // mirror within 8
+    SQ_FOLD(fold<0x4E>, , lane & 2) v[0] += dpp<0x4E>(v[0]);    // quads: 2 3 0 1
+    SQ_FOLD(fold<0xB1>, , lane & 1) v[0] += dpp<0xB1>(v[0]);    // quads: 1 0 3 2
+#undef SQ_FOLD
     return v[0];
 }
 
 // The adjoint that each chunk but the first hands to the one before it when nothing comes in from behind:
 //   g_t = carry + C_t dyg_t, carry = exp(D_t A) g_t, from the chunk's last row to its first
-template <typename T, int NB, int SB>
+template <typename T, int NS>
 __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
-    constexpr int NS = NB * SB;
+    constexpr int U = NS <= 4 ? 4 : NS <= 8 ? 2 : 1;
     __shared__ float2 sd[TS][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cb = blockIdx.x % q.nCb, rest = blockIdx.x / q.nCb;
-    const int chunk = 1 + rest % (q.chunks - 1), b = rest / (q.chunks - 1);
-    const int g = cb / q.cbg, din = (cb % q.cbg) * 64 + lane;
-    const bool ok = din < q.Cg;
-    const int d = g * q.Cg + (ok ? din : q.Cg - 1);
-    const int len = sq_len(p.lengths, b, p.T);
+    const Place x = place(q, q.chunks - 1, 1, p.G, p.T, p.lengths);
+    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f;
     float A2[NS], c[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int n = state_of(w, s / NB, s % NB, NB);
+        const int n = w * NS + s;
         A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
         c[s] = 0.f;
     }
-    const T* dp = (const T*)p.delta + (size_t)b * p.delta_bs + d;
-    const T* zp = p.z ? (const T*)p.z + (size_t)b * p.z_bs + d : nullptr;
-    const T* gp = (const T*)p.dy + (size_t)b * p.T * p.C + d;
-    const int tile0 = chunk * q.chunk_tiles, tile1 = min(tile0 + q.chunk_tiles, q.tiles);
-    const size_t mrow = (size_t)p.G * 2 * q.NP;
+    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
+    const T* zp = p.z ? (const T*)p.z + (size_t)x.b * p.z_bs : nullptr;
+    const T* gp = (const T*)p.dy + (size_t)x.b * p.T * p.C;
+    T rd[RPW], rz[RPW], rg[RPW];
     float total = 0.f;
-    for (int tile = tile1 - 1; tile >= tile0; --tile) {
-        uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((size_t)b * q.Tp + (size_t)tile * TS) * mrow + (size_t)g * 2 * q.NP + (size_t)w * SB * 2 * NB);
+    auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            const int t = min(tile * TS + w * RPW + r, p.T - 1);
+            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
+            rg[r] = (gp + (size_t)t * p.C)[d];
+            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
+        }
+    };
+    load(x.tile1 - 1);
+    float m[2][U][NS];
+    auto fetch = [&](float (&o)[U][NS], uniform_ptr from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) o[i][j] = from[i * 2 * NS + NS + j];
+    };
+    for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
+        uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = ok && t < len;
-            const float raw = (live ? (float)dp[(size_t)t * p.delta_ts] : 0.f) + bias;
-            float step = p.softplus ? sq_softplus(raw) : raw;
-            step = live ? step : 0.f;
-            float dy = live ? (float)gp[(size_t)t * p.C] : 0.f;
-            if (zp) dy *= live ? sq_silu((float)zp[(size_t)t * p.z_ts]) : 0.f;
+            const bool live = x.ok && t < len;
+            const float raw = (float)rd[r] + bias;
+            const float step = live ? p.softplus ? sq_softplus(raw) : raw : 0.f;
+            float dy = (float)rg[r];
+            if (zp) dy *= sq_silu((float)rz[r]);
             total += step;
-            sd[row][lane] = make_float2(step, dy);
+            sd[row][lane] = make_float2(step, live ? dy : 0.f);
         }
+        fetch(m[0], mp + (TS - U) * 2 * NS);
         __syncthreads();
+        if (tile > x.tile0) load(tile - 1);
+        float2 v[2][U];
 #pragma unroll
-        for (int t = TS - 1; t >= 0; --t) {
-            const float2 v = sd[t][lane];
+        for (int i = 0; i < U; ++i) v[0][i] = sd[TS - U + i][lane];
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
-                c[s] = __builtin_amdgcn_exp2f(v.x * A2[s]) * fmaf(mp[t * mrow + (s / NB) * 2 * NB + NB + s % NB], v.y, c[s]);
+        for (int k = 0; k < TS / U; ++k) {
+            if (k + 1 < TS / U) {
+                fetch(m[(k + 1) & 1], mp + (TS - (k + 2) * U) * 2 * NS);
+#pragma unroll
+                for (int i = 0; i < U; ++i) v[(k + 1) & 1][i] = sd[TS - (k + 2) * U + i][lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = U - 1; i >= 0; --i) {
+                const float2 o = v[k & 1][i];
+#pragma unroll
+                for (int s = 0; s < NS; ++s) c[s] = __builtin_amdgcn_exp2f(o.x * A2[s]) * fmaf(m[k & 1][i][s], o.y, c[s]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     }
-    const size_t e = (size_t)b * q.chunks + chunk;
-    if (ok) {
+    const size_t e = (size_t)x.b * q.chunks + x.chunk;
+    if (x.ok) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + state_of(w, s / NB, s % NB, NB)) * p.C + d] = c[s];
+        for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + w * NS + s) * p.C + d] = c[s];
     }
     sd[w][lane].x = total;
     __syncthreads();
-    if (w == 0 && ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
+    if (w == 0 && x.ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
 }
 
 // Per tile, from the last to the first: the states again from the one saved at the tile's start (kept in registers, with the decays), then
-// the adjoint backwards through them.
-template <typename T, int NB, int SB>
-__global__ __launch_bounds__(256) void scan_bwd_kernel(BwdArgs a) {
+// the adjoint backwards through them; NB states of a wave at a time.
+template <typename T, int NS>
+__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
-    constexpr int NS = NB * SB;
-    __shared__ float2 sd[TS][64];      // step, step * u
-    __shared__ float sg[TS][64];       // dy * gate
-    __shared__ float sy[4][TS][64];    // <C, h> over a wave's states
-    __shared__ float2 ss[4][TS][64];   // <g, B>, <g a h_prev, A>
-    __shared__ float sm[TS][4 * SB * 2 * NB];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cb = blockIdx.x % q.nCb, rest = blockIdx.x / q.nCb;
-    const int chunk = rest % q.chunks, b = rest / q.chunks;
-    const int g = cb / q.cbg, din = (cb % q.cbg) * 64 + lane;
-    const bool ok = din < q.Cg;
-    const int d = g * q.Cg + (ok ? din : q.Cg - 1);
-    const int len = sq_len(p.lengths, b, p.T);
+    constexpr int NB = NS < 4 ? NS : 4, U = 2;
+    __shared__ float2 sd[TS][64];     // step, step * u
+    __shared__ float sg[TS][64];      // dy * gate
+    __shared__ float sy[4][TS][64];   // <C, h> over a wave's states
+    __shared__ float2 ss[4][TS][64];  // <g, B>, <g a h_prev, A>
+    __shared__ float sm[4][TS][2 * NS];
+    const Place x = place(q, q.chunks, 0, p.G, p.T, p.lengths);
+    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
     float A2[NS], c[NS], dA[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int n = state_of(w, s / NB, s % NB, NB);
+        const int n = w * NS + s;
         A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
-        c[s] = p.dlast && n < p.N && ok ? p.dlast[((size_t)b * p.C + d) * p.N + n] : 0.f;
+        c[s] = p.dlast && n < p.N && x.ok ? p.dlast[((size_t)x.b * p.C + d) * p.N + n] : 0.f;
         dA[s] = 0.f;
     }
-    for (int k = q.chunks - 1; k > chunk; --k) {
-        const size_t e = (size_t)b * q.chunks + k;
-        const float sum = p.ends_step[e * p.C + d];
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-            c[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), c[s], p.ends[(e * q.NP + state_of(w, s / NB, s % NB, NB)) * p.C + d]);
-    }
-    const T* up = (const T*)p.u + (size_t)b * p.u_bs + d;
-    const T* dp = (const T*)p.delta + (size_t)b * p.delta_bs + d;
-    const T* zp = p.z ? (const T*)p.z + (size_t)b * p.z_bs + d : nullptr;
-    const size_t orow = (size_t)b * p.T * p.C + d;
+    const T* up = (const T*)p.u + (size_t)x.b * p.u_bs;
+    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
+    const T* zp = p.z ? (const T*)p.z + (size_t)x.b * p.z_bs : nullptr;
+    const size_t orow = (size_t)x.b * p.T * p.C;
     const T* gp = (const T*)p.dy + orow;
-    const int tile0 = chunk * q.chunk_tiles, tile1 = min(tile0 + q.chunk_tiles, q.tiles);
-    const size_t mrow = (size_t)p.G * 2 * q.NP;
+    T ru[RPW], rd[RPW], rz[RPW], rg[RPW];
+    auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            const int t = min(tile * TS + w * RPW + r, p.T - 1);
+            ru[r] = (up + (size_t)t * p.u_ts)[d];
+            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
+            rg[r] = (gp + (size_t)t * p.C)[d];
+            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
+        }
+    };
+    load(x.tile1 - 1);
+    chain<NS>(c, A2, p.ends, p.ends_step, q, p.C, x.b, w, d, q.chunks - 1, -1, q.chunks - 1 - x.chunk);
     float dD = 0.f, dbias = 0.f;
-    for (int tile = tile1 - 1; tile >= tile0; --tile) {
-        uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((size_t)b * q.Tp + (size_t)tile * TS) * mrow + (size_t)g * 2 * q.NP + (size_t)w * SB * 2 * NB);
-        float cu[RPW], craw[RPW], cz[RPW], cdy[RPW], cstep[RPW], cg[RPW];
+    for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
+        uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
+        const float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS) * p.C;
+        float cu[RPW], craw[RPW], cz[RPW], cdy[RPW], cstep[RPW], cg[RPW], h0[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) h0[s] = (hp + (size_t)s * p.C)[d];
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = ok && t < len;
-            cu[r] = live ? (float)up[(size_t)t * p.u_ts] : 0.f;
-            craw[r] = (live ? (float)dp[(size_t)t * p.delta_ts] : 0.f) + bias;
-            cdy[r] = live ? (float)gp[(size_t)t * p.C] : 0.f;
-            cz[r] = zp && live ? (float)zp[(size_t)t * p.z_ts] : 0.f;
-            const float step = p.softplus ? sq_softplus(craw[r]) : craw[r];
-            cstep[r] = live ? step : 0.f;
+            const bool live = x.ok && t < len;
+            craw[r] = (float)rd[r] + bias;
+            cstep[r] = live ? p.softplus ? sq_softplus(craw[r]) : craw[r] : 0.f;
+            cu[r] = live ? (float)ru[r] : 0.f;
+            cdy[r] = live ? (float)rg[r] : 0.f;
+            cz[r] = zp && live ? (float)rz[r] : 0.f;
             cg[r] = zp ? cdy[r] * sq_silu(cz[r]) : cdy[r];
             sd[row][lane] = make_float2(cstep[r], cstep[r] * cu[r]);
             sg[row][lane] = cg[r];
         }
         __syncthreads();
+        if (tile > x.tile0) load(tile - 1);
 #pragma unroll
-        for (int sb = 0; sb < SB; ++sb) {
-            float h0[NB], h[TS][NB], av[TS][NB];
+        for (int sb = 0; sb < NS / NB; ++sb) {
+            float h[TS][NB], av[TS][NB];
+            float m[2][U][2 * NB];
+            float2 v[2][U];
+            auto fetch = [&](int set, int t0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const int n = state_of(w, sb, j, NB);
-                h0[j] = n < p.N ? p.hs[(((size_t)b * q.tiles + tile) * p.N + n) * p.C + d] : 0.f;
-            }
+                for (int i = 0; i < U; ++i) {
 #pragma unroll
-            for (int t = 0; t < TS; ++t) {
-                const float2 v = sd[t][lane];
-                float y = sb && zp ? sy[w][t][lane] : 0.f;
-#pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    av[t][j] = __builtin_amdgcn_exp2f(v.x * A2[sb * NB + j]);
-                    h[t][j] = fmaf(av[t][j], t ? h[t - 1][j] : h0[j], v.y * mp[t * mrow + sb * 2 * NB + j]);
-                    y = fmaf(mp[t * mrow + sb * 2 * NB + NB + j], h[t][j], y);
+                    for (int j = 0; j < NB; ++j) {
+                        m[set][i][j] = mp[(t0 + i) * 2 * NS + sb * NB + j];
+                        m[set][i][NB + j] = mp[(t0 + i) * 2 * NS + NS + sb * NB + j];
+                    }
+                    v[set][i] = sd[t0 + i][lane];
                 }
-                if (zp) sy[w][t][lane] = y;
-            }
+            };
+            fetch(0, 0);
 #pragma unroll
-            for (int t = TS - 1; t >= 0; --t) {
-                const float2 v = sd[t][lane];
-                const float dy = sg[t][lane];
-                float2 s12 = sb ? ss[w][t][lane] : make_float2(0.f, 0.f);
-                float val[2 * NB];
+            for (int k = 0; k < TS / U; ++k) {
+                if (k + 1 < TS / U) fetch((k + 1) & 1, (k + 1) * U);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    const int s = sb * NB + j;
-                    const float gv = fmaf(mp[t * mrow + sb * 2 * NB + NB + j], dy, c[s]);
-                    val[j] = gv * v.y;
-                    val[NB + j] = dy * h[t][j];
-                    s12.x = fmaf(gv, mp[t * mrow + sb * 2 * NB + j], s12.x);
-                    c[s] = av[t][j] * gv;
-                    const float qv = c[s] * (t ? h[t - 1][j] : h0[j]);
-                    s12.y = fmaf(qv, A2[s], s12.y);
-                    dA[s] = fmaf(qv, v.x, dA[s]);
+                for (int i = 0; i < U; ++i) {
+                    const int t = k * U + i;
+                    const float2 o = v[k & 1][i];
+                    const float* mm = m[k & 1][i];
+                    float y = sb && zp ? sy[w][t][lane] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        av[t][j] = __builtin_amdgcn_exp2f(o.x * A2[sb * NB + j]);
+                        h[t][j] = fmaf(av[t][j], t ? h[t - 1][j] : h0[sb * NB + j], o.y * mm[j]);
+                        y = fmaf(mm[NB + j], h[t][j], y);
+                    }
+                    if (zp) sy[w][t][lane] = y;
                 }
-                ss[w][t][lane] = s12;
-                const float sum = lane_sums<2 * NB>(val, lane);
-                constexpr int PER = 64 / (2 * NB);
-                if (lane % PER == 0) sm[t][(w * SB + sb) * 2 * NB + lane / PER] = sum;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float gy[2][U];
+            auto fetch_back = [&](int set, int t0) __attribute__((always_inline)) {
+                fetch(set, t0);
+#pragma unroll
+                for (int i = 0; i < U; ++i) gy[set][i] = sg[t0 + i][lane];
+            };
+            fetch_back(0, TS - U);
+            constexpr int PER = 64 / (2 * NB);  // lanes that share a value after the first folds
+#pragma unroll
+            for (int k = 0; k < TS / U; ++k) {
+                if (k + 1 < TS / U) fetch_back((k + 1) & 1, TS - (k + 2) * U);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = U - 1; i >= 0; --i) {
+                    const int t = TS - (k + 1) * U + i;
+                    const float2 o = v[k & 1][i];
+                    const float dy = gy[k & 1][i];
+                    const float* mm = m[k & 1][i];
+                    float2 s12 = sb ? ss[w][t][lane] : make_float2(0.f, 0.f);
+                    float val[2 * NB];
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        const int s = sb * NB + j;
+                        const float gv = fmaf(mm[NB + j], dy, c[s]);
+                        val[j] = gv * o.y;
+                        val[NB + j] = dy * h[t][j];
+                        s12.x = fmaf(gv, mm[j], s12.x);
+                        c[s] = av[t][j] * gv;
+                        const float qv = c[s] * (t ? h[t - 1][j] : h0[s]);
+                        s12.y = fmaf(qv, A2[s], s12.y);
+                        dA[s] = fmaf(qv, o.x, dA[s]);
+                    }
+                    ss[w][t][lane] = s12;
+                    const float sum = lane_sums<2 * NB>(val, lane);
+                    if (lane % PER == 0) {
+                        const int i2 = lane / PER;  // B's share in the first NB, C's in the others
+                        sm[w][t][(i2 / NB) * NS + sb * NB + i2 % NB] = sum;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = ok && t < len;
+            const bool live = x.ok && t < len;
             const float2 x0 = ss[0][row][lane], x1 = ss[1][row][lane], x2 = ss[2][row][lane], x3 = ss[3][row][lane];
             const float s1 = (x0.x + x1.x) + (x2.x + x3.x), s2 = ((x0.y + x1.y) + (x2.y + x3.y)) * SQ_LN2;
             const float du = fmaf(cstep[r], s1, Dd * cg[r]);
@@ -420,37 +525,37 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(BwdArgs a) {
             dd = live ? dd : 0.f;
             dD = fmaf(cg[r], cu[r], dD);
             dbias += dd;
-            if (ok && t < p.T) {
+            if (x.ok && t < p.T) {
                 const size_t o = orow + (size_t)t * p.C;
-                ((T*)p.du)[o] = (T)(live ? du : 0.f);
-                ((T*)p.ddelta)[o] = (T)dd;
+                ((T*)p.du + o)[d] = (T)(live ? du : 0.f);
+                ((T*)p.ddelta + o)[d] = (T)dd;
                 if (zp) {
                     const float y = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                    ((T*)p.dz)[o] = (T)(live ? cdy[r] * y * sq_silu_slope(cz[r]) : 0.f);
+                    ((T*)p.dz + o)[d] = (T)(live ? cdy[r] * y * sq_silu_slope(cz[r]) : 0.f);
                 }
             }
         }
         // this block's share of dB and dC, in the layout of the maps
-        constexpr int MW = 4 * SB * 2 * NB;
-        float* mo = p.dmaps + (size_t)(cb % q.cbg) * ((size_t)p.B * q.Tp * mrow) + ((size_t)b * q.Tp + (size_t)tile * TS) * mrow + (size_t)g * 2 * q.NP;
-        for (int i = threadIdx.x; i < TS * MW; i += 256) mo[(size_t)(i / MW) * mrow + i % MW] = sm[i / MW][i % MW];
+        const int slab = (blockIdx.x % q.nCb) % q.cbg;
+        float* mo = p.dmaps + ((size_t)slab * p.B * p.G * q.tiles + x.item + tile) * (4 * TS * 2 * NS);
+        for (int i = threadIdx.x; i < 4 * TS * 2 * NS; i += 256) mo[i] = (&sm[0][0][0])[i];
         __syncthreads();
     }
-    const size_t e = (size_t)b * q.chunks + chunk;
-    if (ok) {
+    const size_t e = (size_t)x.b * q.chunks + x.chunk;
+    if (x.ok) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) p.dparams[(e * (q.NP + 2) + state_of(w, s / NB, s % NB, NB)) * p.C + d] = dA[s];
-        if (p.dstate && chunk == 0) {
+        for (int s = 0; s < NS; ++s) p.dparams[(e * (q.NP + 2) + w * NS + s) * p.C + d] = dA[s];
+        if (p.dstate && x.chunk == 0) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                const int n = state_of(w, s / NB, s % NB, NB);
-                if (n < p.N) p.dstate[((size_t)b * p.C + d) * p.N + n] = c[s];
+                const int n = w * NS + s;
+                if (n < p.N) p.dstate[((size_t)x.b * p.C + d) * p.N + n] = c[s];
             }
         }
     }
     sd[w][lane] = make_float2(dD, dbias);
     __syncthreads();
-    if (w < 2 && ok) {
+    if (w < 2 && x.ok) {
         const float v = w == 0 ? (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x)
                                : (sd[0][lane].y + sd[1][lane].y) + (sd[2][lane].y + sd[3][lane].y);
         p.dparams[(e * (q.NP + 2) + q.NP + w) * p.C + d] = v;
@@ -461,17 +566,16 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(BwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void scan_dmaps_kernel(const float* __restrict__ dmaps, T* __restrict__ dB, T* __restrict__ dC, Plan q, int B,
                                                          int Tn, int N, int G) {
-    const size_t total = (size_t)B * Tn * G * N, slab = (size_t)B * q.Tp * G * 2 * q.NP;
+    const size_t total = (size_t)B * Tn * G * N, slab = (size_t)B * G * q.tiles * TS * 2 * q.NP;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
         const int n = (int)(i % N);
         const size_t row = i / N;
         const int g = (int)(row % G);
         const size_t bt = row / G;
         const int t = (int)(bt % Tn), b = (int)(bt / Tn);
-        const int sb = n / (4 * q.NB), w = (n / q.NB) % 4, j = n % q.NB;
-        const float* s = dmaps + (((size_t)b * q.Tp + t) * G + g) * 2 * q.NP + (size_t)(w * q.SB + sb) * 2 * q.NB + j;
+        const float* s = dmaps + ((((size_t)b * G + g) * q.tiles + t / TS) * 4 + n / q.NS) * (TS * 2 * q.NS) + (t % TS) * 2 * q.NS + n % q.NS;
         float x = 0.f, y = 0.f;
-        for (int k = 0; k < q.cbg; ++k, s += slab) { x += s[0]; y += s[q.NB]; }
+        for (int k = 0; k < q.cbg; ++k, s += slab) { x += s[0]; y += s[q.NS]; }
         dB[i] = (T)x;
         dC[i] = (T)y;
     }
@@ -548,7 +652,7 @@ int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
     if (B < 1 || T < 1 || C < 1 || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
+    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
 }
 
@@ -557,41 +661,41 @@ int grid_for(size_t n) {
     return (int)(g < 4096 ? g : 4096);
 }
 
-template <typename T, int NB, int SB>
+template <typename T, int NS>
 int launch_fwd(const Args& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_fwd_kernel<T, NB, SB, true><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_fwd_kernel<T, NS, true><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    scan_fwd_kernel<T, NB, SB, false><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    scan_fwd_kernel<T, NS, false><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
 
-template <typename T, int NB, int SB>
+template <typename T, int NS>
 int launch_bwd(const BwdArgs& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_bwd_ends_kernel<T, NB, SB><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_bwd_ends_kernel<T, NS><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    scan_bwd_kernel<T, NB, SB><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    scan_bwd_kernel<T, NS><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
 
-#define SCAN_DISPATCH(FN, T, ARGS)                        \
-    (ARGS.q.SB == 4   ? FN<T, 4, 4>(ARGS, s)              \
-     : ARGS.q.SB == 2 ? FN<T, 4, 2>(ARGS, s)              \
-     : ARGS.q.NB == 4 ? FN<T, 4, 1>(ARGS, s)              \
-     : ARGS.q.NB == 2 ? FN<T, 2, 1>(ARGS, s)              \
-                      : FN<T, 1, 1>(ARGS, s))
+#define SCAN_DISPATCH(FN, T, ARGS)                 \
+    (ARGS.q.NS == 16  ? FN<T, 16>(ARGS, s)         \
+     : ARGS.q.NS == 8 ? FN<T, 8>(ARGS, s)          \
+     : ARGS.q.NS == 4 ? FN<T, 4>(ARGS, s)          \
+     : ARGS.q.NS == 2 ? FN<T, 2>(ARGS, s)          \
+                      : FN<T, 1>(ARGS, s))
 
 template <typename T>
 int fwd(const Args& a, hipStream_t s) {
     const ga_scan_params& p = a.p;
-    scan_maps_kernel<T><<<grid_for((size_t)p.B * a.q.Tp * p.G * a.q.NP), 256, 0, s>>>((const T*)p.Bm, (const T*)p.Cm, p.maps, p.lengths, a.q, p.B, p.T,
+    scan_maps_kernel<T><<<grid_for((size_t)p.B * p.G * a.q.tiles * TS * a.q.NP), 256, 0, s>>>((const T*)p.Bm, (const T*)p.Cm, p.maps, p.lengths, a.q, p.B, p.T,
                                                                                     p.N, p.G, p.b_bs, p.b_ts, p.c_bs, p.c_ts);
     GA_CHECK_LAUNCH();
     return SCAN_DISPATCH(launch_fwd, T, a);
@@ -617,8 +721,8 @@ extern "C" {
 int ga_scan_sizes(int B, int T, int C, int N, int G, ga_scan_buffers* h_out) {
     if (!h_out || bad_sizes(B, T, C, N, G, GA_DTYPE_F32)) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    h_out->maps = (size_t)B * q.Tp * G * 2 * q.NP;
-    h_out->hs = (size_t)B * q.tiles * N * C;
+    h_out->maps = (size_t)B * G * q.tiles * TS * 2 * q.NP;
+    h_out->hs = (size_t)B * q.tiles * q.NP * C;
     h_out->ends = q.chunks > 1 ? (size_t)B * q.chunks * q.NP * C : 0;
     h_out->ends_step = q.chunks > 1 ? (size_t)B * q.chunks * C : 0;
     h_out->dmaps = h_out->maps * q.cbg;

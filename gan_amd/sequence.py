@@ -17,6 +17,7 @@ Sizes and types are checked here (ValueError / TypeError); like every operator o
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
@@ -31,7 +32,7 @@ Tensor = torch.Tensor
 def _act(name: str, t: Optional[Tensor], shape, dtype=None) -> None:
     if t is None:
         return
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
@@ -47,20 +48,23 @@ def _lengths(t: Optional[Tensor], B: int) -> None:
 
 
 def _one_device(first: Tensor, *ts) -> None:
-    L.require_cuda(first, *ts)
+    dev = first.device
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"all tensors of a call must be on one device: got {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            L.require_cuda(first, t)
+            raise RuntimeError(f"all tensors of a call must be on one device: got {dev} and {t.device}")
+    L.require_cuda(first)
 
 
 def _rows(t: Optional[Tensor]) -> Optional[Tensor]:
     """`t` with unit stride along its last axis (itself where it has that already)."""
-    return t if t is None or (t.stride(-1) == 1 and min(t.stride()) >= 0) or t.numel() == 0 else t.contiguous()
+    return t if t is None or t.stride()[-1] == 1 else t.contiguous()
 
 
 def _maps(t: Tensor) -> Tensor:
     """[..., G, N] with the last two axes packed."""
-    return t if t.stride(-1) == 1 and (t.shape[-2] == 1 or t.stride(-2) == t.shape[-1]) and min(t.stride()) >= 0 else t.contiguous()
+    st = t.stride()
+    return t if st[-1] == 1 and (t.shape[-2] == 1 or st[-2] == t.shape[-1]) else t.contiguous()
 
 
 def _packed(t: Optional[Tensor]) -> Optional[Tensor]:
@@ -68,16 +72,24 @@ def _packed(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 def _call(name: str, dev: torch.device, *args) -> None:
+    """One entry of the C ABI on the current stream of `dev`.  (torch.cuda.current_stream builds a Stream object: 5 us of a call that takes 15.)"""
     fn = getattr(L.lib(), name)
-    if dev.index == torch.cuda.current_device():
-        L.check(fn(*args, L.stream()), name)
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            L.check(fn(*args, L.stream()), name)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        L.check(rc, name)
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_grad_step(name: str, whole: str, *ts) -> None:
@@ -205,67 +217,76 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
 
 
 # ------------------------------------------------------------------------------------------------ selective scan
+@lru_cache(maxsize=256)
 def _scan_sizes(B, T, Cn, N, G):
+    """(maps, hs, ends, ends_step, dmaps, dparams): elements of ga_scan_buffers, each rounded up to 16 bytes"""
     s = L.ScanBuffers()
     L.check(L.lib().ga_scan_sizes(B, T, Cn, N, G, C.byref(s)), "ga_scan_sizes")
-    return s
+    return tuple((n + 3) & ~3 for n in (s.maps, s.hs, s.ends, s.ends_step, s.dmaps, s.dparams))
 
 
-def _f32(n: int, dev) -> Optional[Tensor]:
-    return torch.empty((n,), device=dev, dtype=torch.float32) if n else None
-
-
-def _strides(t: Optional[Tensor]):
-    return (0, 0) if t is None else (t.stride(0), t.stride(1))
+def _f32(n: int, dev) -> Tensor:
+    return torch.empty((n,), device=dev, dtype=torch.float32)
 
 
 def _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, softplus, state, lengths, want_last, want_hs):
     B, T, Cn = u.shape
     G, N = Bm.shape[2:]
     dev = u.device
-    s = _scan_sizes(B, T, Cn, N, G)
+    n_maps, n_hs, n_ends, n_step, _, _ = _scan_sizes(B, T, Cn, N, G)
     y = torch.empty((B, T, Cn), device=dev, dtype=u.dtype)
     last = torch.empty((B, Cn, N), device=dev, dtype=torch.float32) if want_last else None
-    maps, hs, ends, ends_step = _f32(s.maps, dev), _f32(s.hs, dev) if want_hs else None, _f32(s.ends, dev), _f32(s.ends_step, dev)
+    keep = _f32(n_maps + n_hs if want_hs else n_maps + n_ends + n_step, dev)  # maps and hs for the backward pass, or maps and what ends here
+    maps = keep.data_ptr()
+    hs = maps + 4 * n_maps if want_hs else 0
+    ends = 0
+    if n_ends:
+        tmp = _f32(n_ends + n_step, dev) if want_hs else None
+        ends = maps + 4 * n_maps if tmp is None else tmp.data_ptr()
     p = L.ScanParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
-                     L.ptr(state), L.ptr(lengths), y.data_ptr(), L.ptr(last), maps.data_ptr(), L.ptr(hs), L.ptr(ends), L.ptr(ends_step),
-                     *_strides(u), *_strides(delta), *_strides(z), *_strides(Bm), *_strides(Cm), B, T, Cn, N, G, int(softplus))
+                     L.ptr(state), L.ptr(lengths), y.data_ptr(), L.ptr(last), maps, hs, ends, ends + 4 * n_ends, *u.stride()[:2], *delta.stride()[:2],
+                     *((0, 0) if z is None else z.stride()[:2]), *Bm.stride()[:2], *Cm.stride()[:2], B, T, Cn, N, G, softplus)
     _call("ga_scan_fwd", dev, C.byref(p), L.dt(u))
-    return y, last, maps, hs
+    return y, last, keep
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, Bm, Cm, D, z, delta_bias, state, softplus, lengths, want_last):
         ctx.set_materialize_grads(False)
-        y, last, maps, hs = _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, softplus, state, lengths, want_last, True)
-        ctx.save_for_backward(u, delta, A, D, z, delta_bias, lengths, maps, hs)
-        ctx.cfg = (tuple(Bm.shape), softplus, state is not None)
+        y, last, keep = _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, softplus, state, lengths, want_last, True)
+        ctx.save_for_backward(u, delta, A, D, z, delta_bias, lengths, keep)
+        ctx.cfg = (*Bm.shape, softplus, state is not None)
         return y, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
-        u, delta, A, D, z, delta_bias, lengths, maps, hs = ctx.saved_tensors
-        (B, T, G, N), softplus, has_state = ctx.cfg
+        u, delta, A, D, z, delta_bias, lengths, keep = ctx.saved_tensors
+        B, T, G, N, softplus, has_state = ctx.cfg
         if dy is None and dlast is None:
             return (None,) * 12
         Cn, dev, dt = u.shape[2], u.device, u.dtype
         dy = torch.zeros((B, T, Cn), device=dev, dtype=dt) if dy is None else dy.contiguous()
         dlast = _packed(dlast)
-        s = _scan_sizes(B, T, Cn, N, G)
-        du, ddelta = torch.empty((2, B, T, Cn), device=dev, dtype=dt).unbind(0)
+        n_maps, _, n_ends, n_step, n_dmaps, n_dparams = _scan_sizes(B, T, Cn, N, G)
+        du = torch.empty((B, T, Cn), device=dev, dtype=dt)
+        ddelta = torch.empty((B, T, Cn), device=dev, dtype=dt)
         dz = torch.empty((B, T, Cn), device=dev, dtype=dt) if z is not None else None
-        dB, dC = torch.empty((2, B, T, G, N), device=dev, dtype=dt).unbind(0)
+        dB = torch.empty((B, T, G, N), device=dev, dtype=dt)
+        dC = torch.empty((B, T, G, N), device=dev, dtype=dt)
         dA = torch.empty((Cn, N), device=dev, dtype=torch.float32)
         dD = _f32(Cn, dev) if D is not None else None
         dbias = _f32(Cn, dev) if delta_bias is not None else None
         dstate = torch.empty((B, Cn, N), device=dev, dtype=torch.float32) if has_state else None
-        ends, ends_step, dmaps, dparams = (_f32(n, dev) for n in (s.ends, s.ends_step, s.dmaps, s.dparams))
+        ws = _f32(n_ends + n_step + n_dmaps + n_dparams, dev)
+        ends = ws.data_ptr()
+        step, maps = ends + 4 * n_ends, keep.data_ptr()
+        dmaps = step + 4 * n_step
         p = L.ScanBwdParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), A.data_ptr(), L.ptr(D), L.ptr(delta_bias), L.ptr(lengths), dy.data_ptr(),
-                            L.ptr(dlast), maps.data_ptr(), hs.data_ptr(), du.data_ptr(), ddelta.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr(),
-                            dA.data_ptr(), L.ptr(dD), L.ptr(dbias), L.ptr(dstate), L.ptr(ends), L.ptr(ends_step), dmaps.data_ptr(),
-                            dparams.data_ptr(), *_strides(u), *_strides(delta), *_strides(z), B, T, Cn, N, G, int(softplus))
+                            L.ptr(dlast), maps, maps + 4 * n_maps, du.data_ptr(), ddelta.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr(),
+                            dA.data_ptr(), L.ptr(dD), L.ptr(dbias), L.ptr(dstate), ends, step, dmaps, dmaps + 4 * n_dmaps, *u.stride()[:2],
+                            *delta.stride()[:2], *((0, 0) if z is None else z.stride()[:2]), B, T, Cn, N, G, softplus)
         _call("ga_scan_bwd", dev, C.byref(p), L.dt(u))
         return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None
 
@@ -319,9 +340,9 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Tensor, 
     u, delta, z, Bm, Cm = _rows(u), _rows(delta), _rows(z), _maps(Bm), _maps(Cm)
     A, D, delta_bias, state, lengths = _packed(A), _packed(D), _packed(delta_bias), _packed(state), _packed(lengths)
     if _wants_grad(u, delta, A, Bm, Cm, D, z, delta_bias, state):
-        y, last = _SelectiveScan.apply(u, delta, A, Bm, Cm, D, z, delta_bias, state, bool(softplus), lengths, bool(return_state))
+        y, last = _SelectiveScan.apply(u, delta, A, Bm, Cm, D, z, delta_bias, state, int(bool(softplus)), lengths, bool(return_state))
     else:
-        y, last, _, _ = _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, bool(softplus), state, lengths, bool(return_state), False)
+        y, last, _ = _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, int(bool(softplus)), state, lengths, bool(return_state), False)
     return (y, last) if return_state else y
 
 

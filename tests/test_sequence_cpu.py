@@ -176,7 +176,7 @@ def test_c_entries_refuse_bad_sizes_without_a_launch():
     for bad in [(0, 1, 1, 1, 1), (1, 0, 1, 1, 1), (1, 1, 6, 65, 1), (1, 1, 6, 4, 4), (1, 1, 6, 0, 1)]:
         assert lib.ga_scan_sizes(*bad, C.byref(s)) == 1
     assert lib.ga_scan_sizes(2, 40, 70, 20, 2, C.byref(s)) == 0
-    assert s.maps == 2 * 48 * 2 * 2 * 32 and s.hs == 2 * 3 * 20 * 70 and s.dmaps == s.maps  # 35 channels of a group: one block of 64
+    assert s.maps == 2 * 48 * 2 * 2 * 32 and s.hs == 2 * 3 * 32 * 70 and s.dmaps == s.maps  # 35 channels of a group: one block of 64
     assert lib.ga_scan_sizes(2, 40, 70, 20, 2, None) == 1
     one = 1 << 20  # a non-null address that no refusal reads
     for fn, P in (("ga_scan_fwd", L.ScanParams), ("ga_scan_bwd", L.ScanBwdParams), ("ga_scan_step", L.ScanStepParams), ("ga_causal_conv_fwd", L.CausalConvParams),
