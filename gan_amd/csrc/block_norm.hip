@@ -10,16 +10,10 @@
 
 namespace {
 
-constexpr int MAX_PARTS = 1024;
+constexpr int MAX_PARTS = 1024, FWD_PARTS = 2048;
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
-template <typename T, int V>
-__device__ __forceinline__ void ldv(float* o, const T* p) {
-    const Pack<T, V> r = *(const Pack<T, V>*)p;
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = (float)r.v[e];
-}
 template <typename T, int V>
 __device__ __forceinline__ void stv(T* p, const float* v) {
     Pack<T, V> r;
@@ -28,58 +22,47 @@ __device__ __forceinline__ void stv(T* p, const float* v) {
     *(Pack<T, V>*)p = r;
 }
 
-// sums of two values over a row's threads, in every one of them
-template <int G>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2 (*red)[4], int& slot) {
+// sums of K values over the G threads of a row, in every one of them
+template <int G, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[8][16], int& slot) {
+    const int lane = threadIdx.x & 63;
+    const float s = sq_lane_sums<K>(v, lane);  // value k in the lanes from k * 64 / K on
+    if (G == 64) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { v.x += __shfl_xor(v.x, o, 64); v.y += __shfl_xor(v.y, o, 64); }
-    if (G == 64) return v;
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) red[slot][w] = v;
-    __syncthreads();
-    const float2 a = red[slot][0], b = red[slot][1], c = red[slot][2], d = red[slot][3];
-    slot ^= 1;  // the other one next: a wave that is ahead by one sum does not write what another still reads
-    return make_float2((a.x + b.x) + (c.x + d.x), (a.y + b.y) + (c.y + d.y));
-}
-
-// (mean, 1 / sqrt(variance or mean square + eps)) of a row
-template <int G, int P, int V>
-__device__ __forceinline__ float2 row_stats(const float (&v)[P][V], const bool (&in)[P], int C, bool layer, float eps, float2 (*red)[4], int& slot) {
-    float mean = 0.f;
-    if (layer) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += in[i] ? v[i][e] : 0.f;
-        mean = row_sum2<G>(make_float2(s, 0.f), red, slot).x / (float)C;
+        for (int k = 0; k < K; ++k) v[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), k * (64 / K)));
+        return;
     }
-    float s = 0.f;
+    if (lane % (64 / K) == 0) red[slot][lane / (64 / K)][threadIdx.x >> 6] = s;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < P; ++i)
+    for (int k = 0; k < K; ++k) {
+        v[k] = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float t = in[i] ? v[i][e] - mean : 0.f;
-            s = fmaf(t, t, s);
+        for (int i = 0; i < G / 64; i += 4) {
+            const float4 t = *(const float4*)(red[slot][k] + i);
+            v[k] += (t.x + t.y) + (t.z + t.w);
         }
-    const float ms = row_sum2<G>(make_float2(s, 0.f), red, slot).x / (float)C;
-    return make_float2(mean, 1.f / sqrtf(ms + eps));
+    }
+    slot ^= 1;  // the other one next: a wave that is ahead by one sum does not write what another still reads
 }
 
 #define BN_COLUMNS()                                                                  \
     const int tid = G == 64 ? threadIdx.x & 63 : threadIdx.x;                         \
     const int w = G == 64 ? threadIdx.x >> 6 : 0;                                     \
-    constexpr int RPB = 256 / G;                                                      \
-    __shared__ float2 red[2][4];                                                      \
+    constexpr int RPB = G == 64 ? 4 : 1;                                              \
+    __shared__ __attribute__((aligned(16))) float red[2][8][16];                      \
     int slot = 0;                                                                     \
     int col[P];                                                                       \
     bool in[P];                                                                       \
+    const float inv = 1.f / (float)p.C;                                               \
     _Pragma("unroll") for (int i = 0; i < P; ++i) {                                   \
         col[i] = (i * G + tid) * V;                                                   \
         in[i] = col[i] < p.C;                                                         \
+        if (!in[i]) col[i] = 0; /* (read, never used or written) */                   \
     }
 
 #define BN_EACH _Pragma("unroll") for (int i = 0; i < P; ++i) _Pragma("unroll") for (int e = 0; e < V; ++e)
+#define BN_ROWS _Pragma("unroll") for (int j = 0; j < R; ++j)
 
 template <int P, int V>
 __device__ __forceinline__ void load_cols(float (&o)[P][V], const float* p, const int (&col)[P], const bool (&in)[P], float none) {
@@ -89,166 +72,207 @@ __device__ __forceinline__ void load_cols(float (&o)[P][V], const float* p, cons
         for (int e = 0; e < V; ++e) o[i][e] = p && in[i] ? p[col[i] + e] : none;
 }
 template <typename T, int P, int V>
-__device__ __forceinline__ void load_rows(float (&o)[P][V], const T* p, const int (&col)[P], const bool (&in)[P]) {
+__device__ __forceinline__ void load_raw(Pack<T, V> (&o)[P], const T* p, const int (&col)[P]) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        if (in[i]) ldv<T, V>(o[i], p + col[i]);
-        else
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[i][e] = 0.f;
-    }
+    for (int i = 0; i < P; ++i) o[i] = *(const Pack<T, V>*)(p + col[i]);
+}
+template <typename T, int P, int V>
+__device__ __forceinline__ void convert(float (&o)[P][V], const Pack<T, V> (&r)[P]) {
+    BN_EACH o[i][e] = (float)r[i].v[e];
 }
 
-template <typename TX, typename TO, int G, int P, int V>
-__global__ __launch_bounds__(256) void bnorm_fwd_kernel(ga_block_norm_params p, int items, long rows_per_item, int parts) {
+// (mean, 1 / sqrt(variance or mean square + eps)) of R rows; the variance about the mean, in a second sum
+template <int G, int P, int V, int R>
+__device__ __forceinline__ void row_stats(const float (&v)[R][P][V], float (&mean)[R], float (&rstd)[R], const bool (&in)[P], float inv, bool layer,
+                                          float eps, float (*red)[8][16], int& slot) {
+    float s[R];
+    BN_ROWS mean[j] = 0.f;
+    if (layer) {
+        BN_ROWS {
+            s[j] = 0.f;
+            BN_EACH s[j] += in[i] ? v[j][i][e] : 0.f;
+        }
+        row_sums<G, R>(s, red, slot);
+        BN_ROWS mean[j] = s[j] * inv;
+    }
+    BN_ROWS {
+        s[j] = 0.f;
+        BN_EACH {
+            const float t = in[i] ? v[j][i][e] - mean[j] : 0.f;
+            s[j] = fmaf(t, t, s[j]);
+        }
+    }
+    row_sums<G, R>(s, red, slot);
+    BN_ROWS rstd[j] = 1.f / sqrtf(fmaf(s[j], inv, eps));
+}
+
+// G threads a row, P pieces of V columns a thread, R rows at a time: their loads are in flight together and their sums share the exchanges
+template <typename TX, typename TO, int G, int P, int V, int R>
+__global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_fwd_kernel(ga_block_norm_params p, long rows_per_item, int parts) {
     BN_COLUMNS();
     const int item = blockIdx.x / parts, part = blockIdx.x % parts;
-    float wv[P][V], bv[P][V], wp[P][V], bp[P][V], sc[P][V], a1[P][V], sh[P][V];
+    float wv[P][V], bv[P][V], wp[P][V], bp[P][V], sc[P][V], tmp[P][V];
     load_cols(wv, p.w, col, in, 1.f);
     load_cols(bv, p.b, col, in, 0.f);
     if (p.ab) {
-        load_cols(a1, p.ab + (size_t)item * 2 * p.C, col, in, 0.f);
-        load_cols(sh, p.ab + (size_t)item * 2 * p.C + p.C, col, in, 0.f);
-        BN_EACH {
-            const float a = 1.f + a1[i][e];
-            wv[i][e] *= a;
-            bv[i][e] = fmaf(bv[i][e], a, sh[i][e]);
-        }
+        load_cols(tmp, p.ab + (size_t)item * 2 * p.C, col, in, 0.f);
+        BN_EACH { wv[i][e] = fmaf(wv[i][e], tmp[i][e], wv[i][e]); bv[i][e] = fmaf(bv[i][e], tmp[i][e], bv[i][e]); }
+        load_cols(tmp, p.ab + (size_t)item * 2 * p.C + p.C, col, in, 0.f);
+        BN_EACH bv[i][e] += tmp[i][e];
     }
-    if (p.branch) {
-        load_cols(wp, p.wp, col, in, 1.f);
-        load_cols(bp, p.bp, col, in, 0.f);
-        load_cols(sc, p.scale, col, in, 1.f);
-        if (p.gate && !p.gate_rows) {
-            load_cols(a1, (const float*)p.gate + (size_t)item * p.C, col, in, 0.f);
-            BN_EACH sc[i][e] *= a1[i][e];
-        }
+    load_cols(wp, p.branch ? p.wp : nullptr, col, in, 1.f);
+    load_cols(bp, p.branch ? p.bp : nullptr, col, in, 0.f);
+    load_cols(sc, p.branch ? p.scale : nullptr, col, in, 1.f);
+    if (p.gate && !p.gate_rows) {
+        load_cols(tmp, (const float*)p.gate + (size_t)item * p.C, col, in, 0.f);
+        BN_EACH sc[i][e] *= tmp[i][e];
     }
-    for (long k = (long)part * RPB + w; k < rows_per_item + (G == 64 ? 0 : 0); k += (long)parts * RPB) {
-        const size_t row = (size_t)item * rows_per_item + k, off = row * p.C;
-        float r[P][V];
-        load_rows<TX, P, V>(r, (const TX*)p.x + off, col, in);
-        float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+    const size_t row0 = (size_t)item * rows_per_item;
+    for (long k = ((long)part * RPB + w) * R; k < rows_per_item; k += (long)parts * RPB * R) {
+        size_t off[R];
+        Pack<TX, V> xr[R][P];
+        Pack<TO, V> orw[R][P], gr[R][P];
+        BN_ROWS {
+            off[j] = (row0 + min(k + j, rows_per_item - 1)) * p.C;
+            load_raw<TX, P, V>(xr[j], (const TX*)p.x + off[j], col);
+            if (p.branch) load_raw<TO, P, V>(orw[j], (const TO*)p.branch + off[j], col);
+            if (p.gate_rows) load_raw<TO, P, V>(gr[j], (const TO*)p.gate + off[j], col);
+        }
+        float r[R][P][V], om[R], os[R], rm[R], rs[R];
+        BN_ROWS { convert(r[j], xr[j]); om[j] = 0.f; os[j] = 1.f; }
         if (p.branch) {
-            float o[P][V], gt[P][V];
-            load_rows<TO, P, V>(o, (const TO*)p.branch + off, col, in);
-            if (p.gate_rows) load_rows<TO, P, V>(gt, (const TO*)p.gate + off, col, in);
-            if (p.post) {
-                const float2 s = row_stats<G, P, V>(o, in, p.C, p.layer, p.eps, red, slot);
-                st.x = s.x;
-                st.y = s.y;
+            float o[R][P][V];
+            BN_ROWS convert(o[j], orw[j]);
+            if (p.post) row_stats<G, P, V, R>(o, om, os, in, inv, p.layer, p.eps, red, slot);
+            BN_ROWS {
+                BN_EACH {
+                    float n = fmaf((o[j][i][e] - om[j]) * os[j], wp[i][e], bp[i][e]);
+                    if (p.gate_rows) n *= (float)gr[j][i].v[e];
+                    r[j][i][e] = fmaf(sc[i][e], n, r[j][i][e]);
+                }
+                if (k + j < rows_per_item) {
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (in[i]) stv<TX, V>((TX*)p.r + off[j] + col[i], r[j][i]);
+                }
             }
-            BN_EACH {
-                float n = fmaf((o[i][e] - st.x) * st.y, wp[i][e], bp[i][e]);
-                if (p.gate_rows) n *= gt[i][e];
-                r[i][e] = fmaf(sc[i][e], n, r[i][e]);
-            }
+        }
+        row_stats<G, P, V, R>(r, rm, rs, in, inv, p.layer, p.eps, red, slot);
+        BN_ROWS {
+            if (k + j >= rows_per_item) break;
+            BN_EACH r[j][i][e] = fmaf((r[j][i][e] - rm[j]) * rs[j], wv[i][e], bv[i][e]);
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i]) stv<TX, V>((TX*)p.r + off + col[i], r[i]);
+                if (in[i]) stv<TO, V>((TO*)p.y + off[j] + col[i], r[j][i]);
+            if (p.stats && tid == 0) *(float4*)(p.stats + (row0 + k + j) * 4) = make_float4(om[j], os[j], rm[j], rs[j]);
         }
-        const float2 s = row_stats<G, P, V>(r, in, p.C, p.layer, p.eps, red, slot);
-        st.z = s.x;
-        st.w = s.y;
-        BN_EACH r[i][e] = fmaf((r[i][e] - s.x) * s.y, wv[i][e], bv[i][e]);
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (in[i]) stv<TO, V>((TO*)p.y + off + col[i], r[i]);
-        if (p.stats && tid == 0) *(float4*)(p.stats + row * 4) = st;
     }
 }
 
-template <typename TX, typename TO, int G, int P, int V>
-__global__ __launch_bounds__(256) void bnorm_bwd_kernel(ga_block_norm_bwd_params p, int items, long rows_per_item, int parts) {
+template <typename TX, typename TO, int G, int P, int V, int R>
+__global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_bwd_kernel(ga_block_norm_bwd_params p, long rows_per_item, int parts) {
     BN_COLUMNS();
     __shared__ float fold[G == 64 ? 4 : 1][G == 64 ? 64 * P * V : 1];
     const int item = blockIdx.x / parts, part = blockIdx.x % parts;
-    const float inv = 1.f / (float)p.C;
     float wv[P][V], wp[P][V], bp[P][V], sc[P][V], tmp[P][V];
     load_cols(wv, p.w, col, in, 1.f);
     if (p.ab) {
         load_cols(tmp, p.ab + (size_t)item * 2 * p.C, col, in, 0.f);
-        BN_EACH wv[i][e] *= 1.f + tmp[i][e];
+        BN_EACH wv[i][e] = fmaf(wv[i][e], tmp[i][e], wv[i][e]);
     }
-    if (p.branch) {
-        load_cols(wp, p.wp, col, in, 1.f);
-        load_cols(bp, p.bp, col, in, 0.f);
-        load_cols(sc, p.scale, col, in, 1.f);
-        if (p.gate && !p.gate_rows) {
-            load_cols(tmp, (const float*)p.gate + (size_t)item * p.C, col, in, 0.f);
-            BN_EACH sc[i][e] *= tmp[i][e];
-        }
+    load_cols(wp, p.branch ? p.wp : nullptr, col, in, 1.f);
+    load_cols(bp, p.branch ? p.bp : nullptr, col, in, 0.f);
+    load_cols(sc, p.branch ? p.scale : nullptr, col, in, 1.f);
+    if (p.gate && !p.gate_rows) {
+        load_cols(tmp, (const float*)p.gate + (size_t)item * p.C, col, in, 0.f);
+        BN_EACH sc[i][e] *= tmp[i][e];
     }
     float s0[P][V], s1[P][V], s2[P][V], s3[P][V];
     BN_EACH s0[i][e] = s1[i][e] = s2[i][e] = s3[i][e] = 0.f;
-    for (long k = (long)part * RPB + w; k < rows_per_item; k += (long)parts * RPB) {
-        const size_t row = (size_t)item * rows_per_item + k, off = row * p.C;
-        const float4 st = *(const float4*)(p.stats + row * 4);
-        float r[P][V], o[P][V], gt[P][V], q[P][V];
-        load_rows<TX, P, V>(r, (const TX*)p.x + off, col, in);
-        if (p.branch) {
-            load_rows<TO, P, V>(o, (const TO*)p.branch + off, col, in);
-            if (p.gate_rows) load_rows<TO, P, V>(gt, (const TO*)p.gate + off, col, in);
-            BN_EACH {
-                o[i][e] = in[i] ? (o[i][e] - st.x) * st.y : 0.f;
-                float n = fmaf(o[i][e], wp[i][e], bp[i][e]);
-                if (p.gate_rows) n *= gt[i][e];
-                r[i][e] = fmaf(sc[i][e], n, r[i][e]);
-            }
+    const size_t row0 = (size_t)item * rows_per_item;
+    for (long k = ((long)part * RPB + w) * R; k < rows_per_item; k += (long)parts * RPB * R) {
+        size_t off[R];
+        bool live[R];
+        Pack<TX, V> xr[R][P], dr[R][P];
+        Pack<TO, V> orw[R][P], gr[R][P], dyr[R][P];
+        float4 st[R];
+        BN_ROWS {
+            live[j] = k + j < rows_per_item;
+            const size_t row = row0 + min(k + j, rows_per_item - 1);
+            off[j] = row * p.C;
+            st[j] = *(const float4*)(p.stats + row * 4);
+            load_raw<TX, P, V>(xr[j], (const TX*)p.x + off[j], col);
+            if (p.branch) load_raw<TO, P, V>(orw[j], (const TO*)p.branch + off[j], col);
+            if (p.gate_rows) load_raw<TO, P, V>(gr[j], (const TO*)p.gate + off[j], col);
+            if (p.dy) load_raw<TO, P, V>(dyr[j], (const TO*)p.dy + off[j], col);
+            if (p.dr) load_raw<TX, P, V>(dr[j], (const TX*)p.dr + off[j], col);
         }
-        BN_EACH q[i][e] = 0.f;
+        float q[R][P][V], o[R][P][V], m[2 * R];
+        BN_ROWS BN_EACH q[j][i][e] = o[j][i][e] = 0.f;
+        if (p.branch) BN_ROWS BN_EACH o[j][i][e] = in[i] ? ((float)orw[j][i].v[e] - st[j].x) * st[j].y : 0.f;
         if (p.dy) {
-            load_rows<TO, P, V>(q, (const TO*)p.dy + off, col, in);
-            float2 m = make_float2(0.f, 0.f);
-            BN_EACH {
-                const float dy = q[i][e];
-                r[i][e] = in[i] ? (r[i][e] - st.z) * st.w : 0.f;
-                s0[i][e] = fmaf(dy, r[i][e], s0[i][e]);
-                s1[i][e] += dy;
-                q[i][e] = dy * wv[i][e];
-                m.x = fmaf(q[i][e], r[i][e], m.x);
-                m.y += q[i][e];
-            }
-            m = row_sum2<G>(m, red, slot);
-            m.x *= inv;
-            m.y = p.layer ? m.y * inv : 0.f;
-            BN_EACH q[i][e] = st.w * (fmaf(-r[i][e], m.x, q[i][e]) - m.y);
-        }
-        if (p.dr) {
-            load_rows<TX, P, V>(r, (const TX*)p.dr + off, col, in);
-            BN_EACH q[i][e] += r[i][e];
-        }
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (in[i]) stv<TX, V>((TX*)p.dx + off + col[i], q[i]);
-        if (p.branch) {
-            float2 m = make_float2(0.f, 0.f);
-            if (p.gate_rows) {
+            float r[R][P][V];
+            BN_ROWS {
+                m[j] = m[R + j] = 0.f;
                 BN_EACH {
-                    const float n = fmaf(o[i][e], wp[i][e], bp[i][e]);
-                    r[i][e] = q[i][e] * sc[i][e] * n;  // the gate's gradient
-                    q[i][e] *= gt[i][e];
+                    float v = (float)xr[j][i].v[e];
+                    if (p.branch) {
+                        float n = fmaf(o[j][i][e], wp[i][e], bp[i][e]);
+                        if (p.gate_rows) n *= (float)gr[j][i].v[e];
+                        v = fmaf(sc[i][e], n, v);
+                    }
+                    v = in[i] && live[j] ? (v - st[j].z) * st[j].w : 0.f;
+                    const float dy = in[i] && live[j] ? (float)dyr[j][i].v[e] : 0.f;
+                    s0[i][e] = fmaf(dy, v, s0[i][e]);
+                    s1[i][e] += dy;
+                    r[j][i][e] = v;
+                    q[j][i][e] = dy * wv[i][e];
+                    m[j] = fmaf(q[j][i][e], v, m[j]);
+                    m[R + j] += q[j][i][e];
                 }
-#pragma unroll
-                for (int i = 0; i < P; ++i)
-                    if (in[i]) stv<TO, V>((TO*)p.dgate + off + col[i], r[i]);
             }
-            BN_EACH {
-                s2[i][e] = fmaf(q[i][e], o[i][e], s2[i][e]);
-                s3[i][e] += q[i][e];
-                q[i][e] *= sc[i][e] * wp[i][e];
-                m.x = fmaf(q[i][e], o[i][e], m.x);
-                m.y += q[i][e];
+            row_sums<G, 2 * R>(m, red, slot);
+            BN_ROWS {
+                const float a = m[j] * inv, b = p.layer ? m[R + j] * inv : 0.f;
+                BN_EACH q[j][i][e] = st[j].w * (fmaf(-r[j][i][e], a, q[j][i][e]) - b);
             }
-            if (p.post) {
-                m = row_sum2<G>(m, red, slot);
-                m.x *= inv;
-                m.y = p.layer ? m.y * inv : 0.f;
-                BN_EACH q[i][e] = st.y * (fmaf(-o[i][e], m.x, q[i][e]) - m.y);
-            }
+        }
+        BN_ROWS {
+            if (p.dr) BN_EACH q[j][i][e] += in[i] && live[j] ? (float)dr[j][i].v[e] : 0.f;
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i]) stv<TO, V>((TO*)p.dbranch + off + col[i], q[i]);
+                if (in[i] && live[j]) stv<TX, V>((TX*)p.dx + off[j] + col[i], q[j][i]);
+        }
+        if (p.branch) {
+            BN_ROWS {
+                m[j] = m[R + j] = 0.f;
+                if (p.gate_rows) {
+                    float dg[P][V];
+                    BN_EACH {
+                        dg[i][e] = q[j][i][e] * sc[i][e] * fmaf(o[j][i][e], wp[i][e], bp[i][e]);
+                        q[j][i][e] *= live[j] ? (float)gr[j][i].v[e] : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (in[i] && live[j]) stv<TO, V>((TO*)p.dgate + off[j] + col[i], dg[i]);
+                }
+                BN_EACH {
+                    const float v = in[i] && live[j] ? q[j][i][e] : 0.f;
+                    s2[i][e] = fmaf(v, o[j][i][e], s2[i][e]);
+                    s3[i][e] += v;
+                    q[j][i][e] = v * (sc[i][e] * wp[i][e]);
+                    m[j] = fmaf(q[j][i][e], o[j][i][e], m[j]);
+                    m[R + j] += q[j][i][e];
+                }
+            }
+            if (p.post) row_sums<G, 2 * R>(m, red, slot);
+            BN_ROWS {
+                const float a = p.post ? m[j] * inv : 0.f, b = p.post && p.layer ? m[R + j] * inv : 0.f;
+                BN_EACH q[j][i][e] = st[j].y * (fmaf(-o[j][i][e], a, q[j][i][e]) - b);
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (in[i] && live[j]) stv<TO, V>((TO*)p.dbranch + off[j] + col[i], q[j][i]);
+            }
         }
     }
     float* out = p.ws + (size_t)blockIdx.x * 4 * p.C;
@@ -267,32 +291,27 @@ __global__ __launch_bounds__(256) void bnorm_bwd_kernel(ga_block_norm_bwd_params
         if (w == 0) {
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i])
-#pragma unroll
-                    for (int e = 0; e < V; ++e) out[(size_t)j * p.C + col[i] + e] = s[i][e];
+                if (in[i]) stv<float, V>(out + (size_t)j * p.C + col[i], s[i]);
         }
     }
 }
 
-// one item's sums over its blocks, and the gradients of its own vectors
+// one item's sums over its blocks, and the gradients of its own vectors; a block is 32 columns
 __global__ __launch_bounds__(256) void bnorm_items_kernel(ga_block_norm_bwd_params p, int parts, float* sums) {
-    __shared__ double acc[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, item = blockIdx.y;
-    const int c = blockIdx.x * 64 + lane;
-    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    __shared__ double acc[4][8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, item = blockIdx.y, c = blockIdx.x * 32 + lane;
     const float* s = p.ws + (size_t)item * parts * 4 * p.C;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (c < p.C)
-            for (int k = w; k < parts; k += 4) v[j] += (double)s[((size_t)k * 4 + j) * p.C + c];
-        __syncthreads();
-        acc[w][lane] = v[j];
-        __syncthreads();
-        v[j] = (acc[0][lane] + acc[1][lane]) + (acc[2][lane] + acc[3][lane]);
-    }
+    for (int j = 0; j < 4; ++j) acc[j][w][lane] = c < p.C ? sq_column(s + (size_t)j * p.C + c, (size_t)4 * p.C, parts, w, 8) : 0.0;
+    __syncthreads();
     if (w || c >= p.C) return;
+    double v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[((size_t)item * 4 + j) * p.C + c] = (float)v[j];
+    for (int j = 0; j < 4; ++j) {
+        v[j] = 0.0;
+        for (int k = 0; k < 8; ++k) v[j] += acc[j][k][lane];
+        sums[((size_t)item * 4 + j) * p.C + c] = (float)v[j];
+    }
     if (p.dab) {
         p.dab[(size_t)item * 2 * p.C + c] = (float)((p.w ? (double)p.w[c] : 1.0) * v[0] + (p.b ? (double)p.b[c] : 0.0) * v[1]);
         p.dab[(size_t)item * 2 * p.C + p.C + c] = (float)v[1];
@@ -302,34 +321,35 @@ __global__ __launch_bounds__(256) void bnorm_items_kernel(ga_block_norm_bwd_para
             (float)((p.scale ? (double)p.scale[c] : 1.0) * ((p.wp ? (double)p.wp[c] : 1.0) * v[2] + (p.bp ? (double)p.bp[c] : 0.0) * v[3]));
 }
 
-// the parameters' gradients from `rows` rows of sums (items when `by_item`, else blocks)
+// the parameters' gradients from `rows` rows of sums (items when `by_item`, else blocks); blockIdx.y: the norm in front / behind
 __global__ __launch_bounds__(1024) void bnorm_params_kernel(ga_block_norm_bwd_params p, const float* sums, int rows, int by_item) {
-    __shared__ double acc[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    __shared__ double acc[32][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, back = blockIdx.y;
+    double v[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (c < p.C)
-            for (int k = w; k < rows; k += 16) {
-                double f = 1.0;
-                if (by_item && j < 2 && p.ab) f += (double)p.ab[(size_t)k * 2 * p.C + c];
-                if (by_item && j >= 2 && p.gate && !p.gate_rows) f = (double)((const float*)p.gate)[(size_t)k * p.C + c];
-                v[j] += f * (double)sums[((size_t)k * 4 + j) * p.C + c];
-            }
-        __syncthreads();
-        acc[w][lane] = v[j];
-        __syncthreads();
+    for (int j = 0; j < 2; ++j) {
+        const float* s = sums + (size_t)(2 * back + j) * p.C + c;
         double t = 0.0;
-        for (int k = 0; k < 16; ++k) t += acc[k][lane];
-        v[j] = t;
+        if (c < p.C) {
+            if (by_item && (back ? p.gate && !p.gate_rows : p.ab != nullptr)) {
+                for (int k = w; k < rows; k += 32) {
+                    const double f = back ? (double)((const float*)p.gate)[(size_t)k * p.C + c] : 1.0 + (double)p.ab[(size_t)k * 2 * p.C + c];
+                    t += f * (double)s[(size_t)k * 4 * p.C];
+                }
+            } else t = sq_column(s, (size_t)4 * p.C, rows, w, 32);
+        }
+        v[j] = sq_groups32(t, acc);
     }
     if (w || c >= p.C) return;
+    if (!back) {
+        if (p.dw) p.dw[c] = (float)v[0];
+        if (p.db) p.db[c] = (float)v[1];
+        return;
+    }
     const double s = p.scale ? (double)p.scale[c] : 1.0, wp = p.wp ? (double)p.wp[c] : 1.0, bp = p.bp ? (double)p.bp[c] : 0.0;
-    if (p.dw) p.dw[c] = (float)v[0];
-    if (p.db) p.db[c] = (float)v[1];
-    if (p.dwp) p.dwp[c] = (float)(s * v[2]);
-    if (p.dbp) p.dbp[c] = (float)(s * v[3]);
-    if (p.dscale) p.dscale[c] = (float)(wp * v[2] + bp * v[3]);
+    if (p.dwp) p.dwp[c] = (float)(s * v[0]);
+    if (p.dbp) p.dbp[c] = (float)(s * v[1]);
+    if (p.dscale) p.dscale[c] = (float)(wp * v[0] + bp * v[1]);
 }
 
 struct Grid {
@@ -360,22 +380,22 @@ int bad(int B, int T, int C, float eps, int xdt, int dt) {
 
 struct Fwd {
     hipStream_t s;
-    template <typename TX, typename TO, int G, int P, int V> int go(const ga_block_norm_params& p) {
-        const Grid g = make_grid(p.B, p.T, p.ab || (p.gate && !p.gate_rows), 256 / G, 2048);
-        bnorm_fwd_kernel<TX, TO, G, P, V><<<(unsigned)(g.items * g.parts), 256, 0, s>>>(p, g.items, g.rows_per_item, g.parts);
+    template <typename TX, typename TO, int G, int P, int V, int R> int go(const ga_block_norm_params& p) {
+        const Grid g = make_grid(p.B, p.T, p.ab || (p.gate && !p.gate_rows), (G == 64 ? 4 : 1) * R, FWD_PARTS);
+        bnorm_fwd_kernel<TX, TO, G, P, V, R><<<(unsigned)(g.items * g.parts), G == 64 ? 256 : G, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();
         return GA_OK;
     }
 };
 struct Bwd {
     hipStream_t s;
-    template <typename TX, typename TO, int G, int P, int V> int go(const ga_block_norm_bwd_params& p) {
+    template <typename TX, typename TO, int G, int P, int V, int R> int go(const ga_block_norm_bwd_params& p) {
         const bool by_item = p.ab || (p.gate && !p.gate_rows);
-        const Grid g = make_grid(p.B, p.T, by_item, 256 / G, MAX_PARTS);
+        const Grid g = make_grid(p.B, p.T, by_item, (G == 64 ? 4 : 1) * R, MAX_PARTS);
         const int blocks = g.items * g.parts;
-        bnorm_bwd_kernel<TX, TO, G, P, V><<<(unsigned)blocks, 256, 0, s>>>(p, g.items, g.rows_per_item, g.parts);
+        bnorm_bwd_kernel<TX, TO, G, P, V, R><<<(unsigned)blocks, G == 64 ? 256 : G, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();
-        const unsigned cb = (unsigned)((p.C + 63) / 64);
+        const unsigned cb = (unsigned)((p.C + 31) / 32);
         const float* sums = p.ws;
         if (by_item) {
             float* items = p.ws + (size_t)blocks * 4 * p.C;
@@ -390,7 +410,7 @@ struct Bwd {
             }
             sums = items;
         }
-        bnorm_params_kernel<<<cb, 1024, 0, s>>>(p, sums, by_item ? g.items : blocks, by_item);
+        bnorm_params_kernel<<<dim3(cb, p.branch ? 2 : 1), 1024, 0, s>>>(p, sums, by_item ? g.items : blocks, by_item);
         GA_CHECK_LAUNCH();
         return GA_OK;
     }
@@ -399,16 +419,17 @@ struct Bwd {
 template <typename TX, typename TO, typename F, typename A>
 int by_width(const A& p, bool vec, F f) {
     if (vec) {
-        if (p.C <= 256) return f.template go<TX, TO, 64, 1, 4>(p);
-        if (p.C <= 512) return f.template go<TX, TO, 64, 2, 4>(p);
-        if (p.C <= 1024) return f.template go<TX, TO, 64, 4, 4>(p);
-        if (p.C <= 2048) return f.template go<TX, TO, 256, 2, 4>(p);
-        if (p.C <= 4096) return f.template go<TX, TO, 256, 4, 4>(p);
-        return f.template go<TX, TO, 256, 8, 4>(p);
+        if (p.C <= 256) return f.template go<TX, TO, 64, 1, 4, 4>(p);
+        if (p.C <= 512) return f.template go<TX, TO, 64, 2, 4, 2>(p);
+        if (p.C <= 1024) return f.template go<TX, TO, 256, 1, 4, 4>(p);
+        if (p.C <= 2048) return f.template go<TX, TO, 256, 2, 4, 2>(p);
+        if (p.C <= 4096) return f.template go<TX, TO, 1024, 1, 4, 2>(p);
+        return f.template go<TX, TO, 1024, 2, 4, 1>(p);
     }
-    if (p.C <= 256) return f.template go<TX, TO, 64, 4, 1>(p);
-    if (p.C <= 1024) return f.template go<TX, TO, 256, 4, 1>(p);
-    return f.template go<TX, TO, 256, 32, 1>(p);
+    if (p.C <= 256) return f.template go<TX, TO, 64, 4, 1, 2>(p);
+    if (p.C <= 1024) return f.template go<TX, TO, 256, 4, 1, 2>(p);
+    if (p.C <= 4096) return f.template go<TX, TO, 1024, 4, 1, 1>(p);
+    return f.template go<TX, TO, 1024, 8, 1, 1>(p);
 }
 template <typename F, typename A>
 int by_type(const A& p, int xdt, int dt, bool vec, F f) {

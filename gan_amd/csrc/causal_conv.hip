@@ -211,16 +211,10 @@ __global__ __launch_bounds__(256) void cconv_bwd_kernel(ga_causal_conv_bwd_param
 
 __global__ __launch_bounds__(1024) void cconv_dw_kernel(const float* __restrict__ ws, int parts, int K, int C, float* __restrict__ dw,
                                                         float* __restrict__ db) {
-    __shared__ double acc[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long col = (long)blockIdx.x * 64 + lane, cols = (long)(K + 1) * C;
-    double v = 0.0;
-    if (col < cols)
-        for (int r = w; r < parts; r += 16) v += (double)ws[(size_t)r * cols + col];
-    acc[w][lane] = v;
-    __syncthreads();
-    if (w == 0 && col < cols) {
-        for (int k = 1; k < 16; ++k) v += acc[k][lane];
+    __shared__ double acc[32][32];
+    const long col = (long)blockIdx.x * 32 + (threadIdx.x & 31), cols = (long)(K + 1) * C;
+    const double v = sq_groups32(col < cols ? sq_column(ws + col, cols, parts, threadIdx.x >> 5, 32) : 0.0, acc);
+    if (threadIdx.x < 32 && col < cols) {
         const int k = (int)(col / C), c = (int)(col % C);
         if (k < K) dw[(size_t)c * K + k] = (float)v;
         else if (db) db[c] = (float)v;
@@ -276,7 +270,7 @@ int bwd(const ga_causal_conv_bwd_params& p, hipStream_t s) {
     const int parts = parts_of(m);
     cconv_bwd_kernel<T, V, K><<<(unsigned)(parts * m.pb), 256, 0, s>>>(p, m, parts);
     GA_CHECK_LAUNCH();
-    cconv_dw_kernel<<<(unsigned)(((long)(K + 1) * p.C + 63) / 64), 1024, 0, s>>>(p.ws, parts, K, p.C, p.dw, p.dbias);
+    cconv_dw_kernel<<<(unsigned)(((long)(K + 1) * p.C + 31) / 32), 1024, 0, s>>>(p.ws, parts, K, p.C, p.dw, p.dbias);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }

@@ -245,44 +245,6 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     }
 }
 
-// Sums over the 64 lanes of many values at once: each step sends one half of the values each way across a lane bit, so that the work halves
-// with it (V values cost 2V - 2 exchanges and adds and not 6V).  permlane swaps for the upper two lane bits, DPP for the others.
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-__device__ __forceinline__ float fold32(float a, float b) {  // lanes 0-31: a over both halves, 32-63: b
-    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
-}
-__device__ __forceinline__ float fold16(float a, float b) {
-    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
-}
-template <int CTRL>
-__device__ __forceinline__ float fold(float a, float b, bool up) {
-    return (up ? b : a) + dpp<CTRL>(up ? a : b);
-}
-// n values (a power of two) in v; lane l leaves with v[0] = the sum of value (the top log2 n bits of l)
-template <int V>
-__device__ __forceinline__ float lane_sums(float (&v)[V], int lane) {
-    static_assert(V >= 1 && V <= 64 && (V & (V - 1)) == 0, "a power of two");
-    int n = V;
-#define SQ_FOLD(FN, ...)                                                              \
-    if (n > 1) {                                                                      \
-        n >>= 1;                                                                      \
-        _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = FN(v[i], v[i + n] __VA_ARGS__); \
-    } else
-    SQ_FOLD(fold32) v[0] = fold32(v[0], v[0]);
-    SQ_FOLD(fold16) v[0] = fold16(v[0], v[0]);
-    SQ_FOLD(fold<0x128>, , lane & 8) v[0] += dpp<0x128>(v[0]);  // rotate by 8 within 16
-    SQ_FOLD(fold<0x141>, , lane & 4) v[0] += dpp<0x141>(v[0]);  // mirror within 8
-    SQ_FOLD(fold<0x4E>, , lane & 2) v[0] += dpp<0x4E>(v[0]);    // quads: 2 3 0 1
-    SQ_FOLD(fold<0xB1>, , lane & 1) v[0] += dpp<0xB1>(v[0]);    // quads: 1 0 3 2
-#undef SQ_FOLD
-    return v[0];
-}
-
 // The adjoint that each chunk but the first hands to the one before it when nothing comes in from behind:
 //   g_t = carry + C_t dyg_t, carry = exp(D_t A) g_t, from the chunk's last row to its first
 template <typename T, int NS>
@@ -503,7 +465,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                         dA[s] = fmaf(qv, o.x, dA[s]);
                     }
                     ss[w][t][lane] = s12;
-                    const float sum = lane_sums<2 * NB>(val, lane);
+                    const float sum = sq_lane_sums<2 * NB>(val, lane);
                     if (lane % PER == 0) {
                         const int i2 = lane / PER;  // B's share in the first NB, C's in the others
                         sm[w][t][(i2 / NB) * NS + sb * NB + i2 % NB] = sum;
@@ -584,16 +546,10 @@ __global__ __launch_bounds__(256) void scan_dmaps_kernel(const float* __restrict
 // dA [C][N], dD, ddelta_bias [C]: the items' and chunks' shares ([rows][NP + 2][C]) added up
 __global__ __launch_bounds__(1024) void scan_dparams_kernel(const float* __restrict__ parts, int rows, int NP, int C, int N, float* __restrict__ dA,
                                                             float* __restrict__ dD, float* __restrict__ dbias) {
-    __shared__ double acc[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long col = (long)blockIdx.x * 64 + lane, cols = (long)(NP + 2) * C;
-    double v = 0.0;
-    if (col < cols)
-        for (int r = w; r < rows; r += 16) v += (double)parts[(size_t)r * cols + col];
-    acc[w][lane] = v;
-    __syncthreads();
-    if (w == 0 && col < cols) {
-        for (int k = 1; k < 16; ++k) v += acc[k][lane];
+    __shared__ double acc[32][32];
+    const long col = (long)blockIdx.x * 32 + (threadIdx.x & 31), cols = (long)(NP + 2) * C;
+    const double v = sq_groups32(col < cols ? sq_column(parts + col, cols, rows, threadIdx.x >> 5, 32) : 0.0, acc);
+    if (threadIdx.x < 32 && col < cols) {
         const int s = (int)(col / C), d = (int)(col % C);
         if (s < N) dA[(size_t)d * N + s] = (float)v;
         else if (s == NP && dD) dD[d] = (float)v;
@@ -709,7 +665,7 @@ int bwd(const BwdArgs& a, hipStream_t s) {
     scan_dmaps_kernel<T><<<grid_for((size_t)p.B * p.T * p.G * p.N), 256, 0, s>>>(p.dmaps, (T*)p.dBm, (T*)p.dCm, a.q, p.B, p.T, p.N, p.G);
     GA_CHECK_LAUNCH();
     const long cols = (long)(a.q.NP + 2) * p.C;
-    scan_dparams_kernel<<<(unsigned)((cols + 63) / 64), 1024, 0, s>>>(p.dparams, p.B * a.q.chunks, a.q.NP, p.C, p.N, p.dA, p.dD, p.ddelta_bias);
+    scan_dparams_kernel<<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(p.dparams, p.B * a.q.chunks, a.q.NP, p.C, p.N, p.dA, p.dD, p.ddelta_bias);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
