@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int MAX_PARTS = 1024, FWD_PARTS = 2048;
+constexpr int MAX_PARTS = 1024;  // blocks of a backward launch at the most, each with a row of sums
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
@@ -356,16 +356,22 @@ struct Grid {
     int items, parts;
     long rows_per_item;
 };
-// without vectors of their own the items are one long item
-Grid make_grid(int B, int T, bool by_item, int rows_per_block, int most) {
+// Without vectors of their own the items are one long item.  As many blocks as fit the card at once (`most`: more leave a last, partly filled
+// round, measured 170 us at three blocks a CU and 227 at four where three fit), and no more than the same number of turns over the rows needs.
+Grid make_grid(int B, int T, bool by_item, int rows_per_turn, int most) {
     Grid g;
     g.items = by_item ? B : 1;
     g.rows_per_item = by_item ? T : (long)B * T;
-    long parts = (g.rows_per_item + rows_per_block - 1) / rows_per_block;
     const long cap = g.items < most ? most / g.items : 1;
-    if (parts > cap) parts = cap;
-    g.parts = (int)parts;
+    const long turns = (g.rows_per_item + cap * rows_per_turn - 1) / (cap * rows_per_turn);
+    g.parts = (int)((g.rows_per_item + turns * rows_per_turn - 1) / (turns * rows_per_turn));
     return g;
+}
+template <typename K>
+int resident_blocks(K kernel, int threads) {
+    int per_cu = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess || per_cu < 1) per_cu = 1;
+    return 256 * (per_cu < 4 ? per_cu : 4);
 }
 
 bool aligned(const void* p, size_t bytes) { return !((uintptr_t)p & (bytes - 1)); }
@@ -380,20 +386,26 @@ int bad(int B, int T, int C, float eps, int xdt, int dt) {
 
 struct Fwd {
     hipStream_t s;
+    static constexpr int R(int fwd, int) { return fwd; }
     template <typename TX, typename TO, int G, int P, int V, int R> int go(const ga_block_norm_params& p) {
-        const Grid g = make_grid(p.B, p.T, p.ab || (p.gate && !p.gate_rows), (G == 64 ? 4 : 1) * R, FWD_PARTS);
-        bnorm_fwd_kernel<TX, TO, G, P, V, R><<<(unsigned)(g.items * g.parts), G == 64 ? 256 : G, 0, s>>>(p, g.rows_per_item, g.parts);
+        constexpr int threads = G == 64 ? 256 : G;
+        static const int most = resident_blocks(bnorm_fwd_kernel<TX, TO, G, P, V, R>, threads);
+        const Grid g = make_grid(p.B, p.T, p.ab || (p.gate && !p.gate_rows), (G == 64 ? 4 : 1) * R, most);
+        bnorm_fwd_kernel<TX, TO, G, P, V, R><<<(unsigned)(g.items * g.parts), threads, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();
         return GA_OK;
     }
 };
 struct Bwd {
     hipStream_t s;
+    static constexpr int R(int, int bwd) { return bwd; }
     template <typename TX, typename TO, int G, int P, int V, int R> int go(const ga_block_norm_bwd_params& p) {
         const bool by_item = p.ab || (p.gate && !p.gate_rows);
-        const Grid g = make_grid(p.B, p.T, by_item, (G == 64 ? 4 : 1) * R, MAX_PARTS);
+        constexpr int threads = G == 64 ? 256 : G;
+        static const int most = resident_blocks(bnorm_bwd_kernel<TX, TO, G, P, V, R>, threads);
+        const Grid g = make_grid(p.B, p.T, by_item, (G == 64 ? 4 : 1) * R, most);
         const int blocks = g.items * g.parts;
-        bnorm_bwd_kernel<TX, TO, G, P, V, R><<<(unsigned)blocks, G == 64 ? 256 : G, 0, s>>>(p, g.rows_per_item, g.parts);
+        bnorm_bwd_kernel<TX, TO, G, P, V, R><<<(unsigned)blocks, threads, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();
         const unsigned cb = (unsigned)((p.C + 31) / 32);
         const float* sums = p.ws;
@@ -419,15 +431,15 @@ struct Bwd {
 template <typename TX, typename TO, typename F, typename A>
 int by_width(const A& p, bool vec, F f) {
     if (vec) {
-        if (p.C <= 256) return f.template go<TX, TO, 64, 1, 4, 4>(p);
-        if (p.C <= 512) return f.template go<TX, TO, 64, 2, 4, 2>(p);
-        if (p.C <= 1024) return f.template go<TX, TO, 256, 1, 4, 4>(p);
-        if (p.C <= 2048) return f.template go<TX, TO, 256, 2, 4, 2>(p);
-        if (p.C <= 4096) return f.template go<TX, TO, 1024, 1, 4, 2>(p);
+        if (p.C <= 256) return f.template go<TX, TO, 64, 1, 4, F::R(4, 2)>(p);
+        if (p.C <= 512) return f.template go<TX, TO, 64, 2, 4, F::R(2, 1)>(p);
+        if (p.C <= 1024) return f.template go<TX, TO, 256, 1, 4, F::R(4, 2)>(p);
+        if (p.C <= 2048) return f.template go<TX, TO, 256, 2, 4, F::R(2, 1)>(p);
+        if (p.C <= 4096) return f.template go<TX, TO, 1024, 1, 4, F::R(2, 1)>(p);
         return f.template go<TX, TO, 1024, 2, 4, 1>(p);
     }
-    if (p.C <= 256) return f.template go<TX, TO, 64, 4, 1, 2>(p);
-    if (p.C <= 1024) return f.template go<TX, TO, 256, 4, 1, 2>(p);
+    if (p.C <= 256) return f.template go<TX, TO, 64, 4, 1, F::R(2, 1)>(p);
+    if (p.C <= 1024) return f.template go<TX, TO, 256, 4, 1, F::R(2, 1)>(p);
     if (p.C <= 4096) return f.template go<TX, TO, 1024, 4, 1, 1>(p);
     return f.template go<TX, TO, 1024, 8, 1, 1>(p);
 }
@@ -443,8 +455,8 @@ extern "C" {
 
 size_t ga_block_norm_bwd_ws_elems(int B, int T, int C, int by_item) {
     if (bad(B, T, C, 1.f, GA_DTYPE_F32, GA_DTYPE_F32)) return 0;
-    const Grid g = make_grid(B, T, by_item != 0, 1, MAX_PARTS);  // one row a block: at least as many as any launch has
-    return ((size_t)g.items * g.parts + (by_item ? (size_t)B : 0)) * 4 * C;
+    const size_t items = by_item ? (size_t)B : 1, rows = by_item ? (size_t)T : (size_t)B * T, cap = items < MAX_PARTS ? MAX_PARTS / items : 1;
+    return (items * (rows < cap ? rows : cap) + (by_item ? items : 0)) * 4 * C;
 }
 
 int ga_block_norm_fwd(const ga_block_norm_params* hp, int xdtype, int dtype, hipStream_t s) {

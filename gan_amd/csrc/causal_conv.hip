@@ -2,24 +2,25 @@
 //   pre[b][t][c] = bias[c] + sum_k w[c][k] x[b][t - (K-1) + k][c],  y = act(pre),  rows before 0 from the window (or zero)
 // forward, backward and the single-token step.  HBM-bound: a few multiply-adds for each element read and written.
 //
-// A thread owns VEC adjacent channels (one 16-byte access a row where alignment allows) and a run of RUN rows, with the last K rows in
-// registers: a row is read once by its run and K - 1 rows of every run again by the next one (from cache, mostly).
+// A thread owns V adjacent channels (one 8- or 16-byte access a row where alignment allows) and a run of rows, the last K of them in registers:
+// slot (K-1 + r) mod K holds the run's row r, so that a turn of K rows moves nothing.  A row is read once by its run and K - 1 rows of every
+// run again by the next one (from cache, mostly); the loads of the next K rows are in flight while K rows are worked on.
 #include "seq_common.h"
 
 namespace {
 
-constexpr int RUN = 16;
 constexpr int MAX_PARTS = 1024;  // blocks along time of the backward pass, each with a row of weight-gradient sums
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 struct Map {
-    int px, ry;     // channel pieces and runs of a block (px * ry = 256)
-    int pieces, pb; // pieces of a row, piece blocks
-    long runs;      // B * runs of an item
-    int rpi;        // runs of an item
+    int px, ry;      // channel pieces and runs of a block (px * ry = 256)
+    int pieces, pb;  // pieces of a row, piece blocks
+    int run, rpi;    // rows of a run, runs of an item
+    long runs;       // of all items
 };
 
+// Runs as long as 1024 blocks (four a CU) allow, 16 to 128 rows: the K - 1 rows read twice are then at most a fifth.
 Map make_map(int B, int T, int C, int vec) {
     Map m;
     m.pieces = (C + vec - 1) / vec;
@@ -27,7 +28,11 @@ Map make_map(int B, int T, int C, int vec) {
     while (m.px > 1 && m.px / 2 >= m.pieces) m.px >>= 1;
     m.ry = 256 / m.px;
     m.pb = (m.pieces + m.px - 1) / m.px;
-    m.rpi = (T + RUN - 1) / RUN;
+    const long blocks_of_one_run = ((long)B * m.pb + m.ry - 1) / m.ry;
+    long want = 1024 / (blocks_of_one_run < 1024 ? blocks_of_one_run : 1024);
+    long run = (T + want - 1) / want;
+    m.run = (int)(run < 16 ? 16 : run > 128 ? 128 : run);
+    m.rpi = (T + m.run - 1) / m.run;
     m.runs = (long)B * m.rpi;
     return m;
 }
@@ -51,7 +56,7 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
     *(Pack<T, V>*)p = r;
 }
 
-// row f of (window ; sequence), f = 0 .. K-2 + len; zero where there is none
+// row t of (window ; sequence), t = -(K-1) .. len - 1; zero where there is none
 template <typename T, int V>
 __device__ __forceinline__ void load_joined(float (&o)[V], const T* x, long x_ts, const T* state, int K, int C, int t, int len) {
     if (t >= 0) load_row<T, V>(o, x + (size_t)t * x_ts, t < len);
@@ -63,11 +68,17 @@ __global__ __launch_bounds__(256) void cconv_fwd_kernel(ga_causal_conv_params p,
     const int px = threadIdx.x % m.px, piece = (blockIdx.x % m.pb) * m.px + px;
     const long run = (long)(blockIdx.x / m.pb) * m.ry + threadIdx.x / m.px;
     if (piece >= m.pieces || run >= m.runs) return;
-    const int b = (int)(run / m.rpi), t0 = (int)(run % m.rpi) * RUN, c0 = piece * V;
-    const int len = sq_len(p.lengths, b, p.T);
+    const int b = (int)(run / m.rpi), t0 = (int)(run % m.rpi) * m.run, c0 = piece * V;
+    const int len = sq_len(p.lengths, b, p.T), rows = min(m.run, p.T - t0);
     const T* x = (const T*)p.x + (size_t)b * p.x_bs + c0;
     const T* st = p.state ? (const T*)p.state + (size_t)b * (K - 1) * p.C + c0 : nullptr;
     T* y = (T*)p.y + ((size_t)b * p.T + t0) * p.C + c0;
+    Pack<T, V> next[K];
+    auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) next[i] = *(const Pack<T, V>*)(x + (size_t)min(t0 + r0 + i, p.T - 1) * p.x_ts);
+    };
+    load(0);
     float w[K][V], bias[V], win[K][V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -77,25 +88,27 @@ __global__ __launch_bounds__(256) void cconv_fwd_kernel(ga_causal_conv_params p,
     }
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) load_joined<T, V>(win[k], x, p.x_ts, st, K, p.C, t0 - (K - 1) + k, len);
+    for (int r0 = 0; r0 < rows; r0 += K) {
+        Pack<T, V> cur[K];
 #pragma unroll
-    for (int r = 0; r < RUN; ++r) {
-        const int t = t0 + r;
-        if (t >= p.T) break;
-        load_row<T, V>(win[K - 1], x + (size_t)t * p.x_ts, t < len);
-        float o[V];
+        for (int i = 0; i < K; ++i) cur[i] = next[i];
+        if (r0 + K < rows) load(r0 + K);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float v = bias[e];
+        for (int i = 0; i < K; ++i) {
+            const int r = r0 + i;
+            const bool live = t0 + r < len;
+            float o[V];
 #pragma unroll
-            for (int k = 0; k < K; ++k) v = fmaf(w[k][e], win[k][e], v);
-            if (p.act == GA_ACT_SILU) v = sq_silu(v);
-            o[e] = t < len ? v : 0.f;
+            for (int e = 0; e < V; ++e) {
+                win[(K - 1 + i) % K][e] = live ? (float)cur[i].v[e] : 0.f;
+                float v = bias[e];
+#pragma unroll
+                for (int k = 0; k < K; ++k) v = fmaf(w[k][e], win[(i + k) % K][e], v);
+                if (p.act == GA_ACT_SILU) v = sq_silu(v);
+                o[e] = live ? v : 0.f;
+            }
+            if (r < rows) store_row<T, V>(y + (size_t)r * p.C, o);
         }
-        store_row<T, V>(y + (size_t)r * p.C, o);
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
     }
     if (p.last && t0 == 0) {
 #pragma unroll
@@ -114,78 +127,92 @@ __global__ __launch_bounds__(256) void cconv_bwd_kernel(ga_causal_conv_bwd_param
     __shared__ float red[256][V];
     const int px = threadIdx.x % m.px, ry = threadIdx.x / m.px, piece = (blockIdx.x % m.pb) * m.px + px;
     const int part = blockIdx.x / m.pb;
-    const int c0 = piece * V;
+    const bool in = piece < m.pieces;
+    const int c0 = in ? piece * V : 0;
     float w[K][V], bias[V], dw[K][V], db[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const bool in = piece < m.pieces;
-        bias[e] = in && p.bias ? p.bias[c0 + e] : 0.f;
+        bias[e] = p.bias ? p.bias[c0 + e] : 0.f;
         db[e] = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            w[k][e] = in ? p.w[(size_t)(c0 + e) * K + k] : 0.f;
+            w[k][e] = p.w[(size_t)(c0 + e) * K + k];
             dw[k][e] = 0.f;
         }
     }
-    if (piece < m.pieces) {
+    if (in) {
         for (long run = (long)part * m.ry + ry; run < m.runs; run += (long)parts * m.ry) {
-            const int b = (int)(run / m.rpi), t0 = (int)(run % m.rpi) * RUN;
-            const int len = sq_len(p.lengths, b, p.T);
+            const int b = (int)(run / m.rpi), t0 = (int)(run % m.rpi) * m.run;
+            const int len = sq_len(p.lengths, b, p.T), rows = min(m.run, p.T - t0);
             const T* x = (const T*)p.x + (size_t)b * p.x_bs + c0;
             const T* st = p.state ? (const T*)p.state + (size_t)b * (K - 1) * p.C + c0 : nullptr;
             const T* gy = (const T*)p.dy + (size_t)b * p.T * p.C + c0;
-            float win[K][V], acc[K][V];  // acc[k]: dx of row t - (K-1) + k so far
+            Pack<T, V> xn[K], gn[K];
+            auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const int t = min(t0 + r0 + i, p.T - 1);
+                    xn[i] = *(const Pack<T, V>*)(x + (size_t)t * p.x_ts);
+                    gn[i] = *(const Pack<T, V>*)(gy + (size_t)t * p.C);
+                }
+            };
+            load(0);
+            float win[K][V], acc[K][V];  // the input's and its gradient's rows t - (K-1) .. t, in the same slots
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e) acc[k][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < K - 1; ++k) load_joined<T, V>(win[k], x, p.x_ts, st, K, p.C, t0 - (K - 1) + k, len);
+            for (int r0 = 0; r0 < rows + K - 1; r0 += K) {
+                Pack<T, V> xc[K], gc[K];
 #pragma unroll
-            for (int r = 0; r < RUN + K - 1; ++r) {
-                const int t = t0 + r;
-                load_row<T, V>(win[K - 1], x + (size_t)t * p.x_ts, t < len);
-                float g[V];
-                load_row<T, V>(g, gy + (size_t)t * p.C, t < len);
+                for (int i = 0; i < K; ++i) { xc[i] = xn[i]; gc[i] = gn[i]; }
+                if (r0 + K < rows + K - 1) load(r0 + K);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if (p.act == GA_ACT_SILU) {
-                        float v = bias[e];
+                for (int i = 0; i < K; ++i) {
+                    const int r = r0 + i, t = t0 + r, ns = (K - 1 + i) % K;
+                    const bool live = t < len, own = r < rows;
 #pragma unroll
-                        for (int k = 0; k < K; ++k) v = fmaf(w[k][e], win[k][e], v);
-                        g[e] = t < len ? g[e] * sq_silu_slope(v) : 0.f;
+                    for (int e = 0; e < V; ++e) {
+                        win[ns][e] = live ? (float)xc[i].v[e] : 0.f;
+                        acc[ns][e] = 0.f;
+                        float g = (float)gc[i].v[e];
+                        if (p.act == GA_ACT_SILU) {
+                            float v = bias[e];
+#pragma unroll
+                            for (int k = 0; k < K; ++k) v = fmaf(w[k][e], win[(i + k) % K][e], v);
+                            g *= sq_silu_slope(v);
+                        }
+                        g = live ? g : 0.f;
+                        const float go = own ? g : 0.f;
+                        db[e] += go;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) {
+                            dw[k][e] = fmaf(go, win[(i + k) % K][e], dw[k][e]);
+                            acc[(i + k) % K][e] = fmaf(w[k][e], g, acc[(i + k) % K][e]);
+                        }
                     }
-                    if (r < RUN) db[e] += g[e];
+                    const int td = t - (K - 1);              // this row of dx is complete
+                    const int from = td - (len - (K - 1));  // its place among the rows handed on as the window
+                    float(&done)[V] = acc[i % K];
+                    if (r < rows + K - 1 && (td >= t0 || t0 == 0)) {
+                        if (p.dlast && from >= 0 && from < K - 1) {
+                            float v[V];
+                            load_row<T, V>(v, (const T*)p.dlast + ((size_t)b * (K - 1) + from) * p.C + c0, true);
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        if (r < RUN) dw[k][e] = fmaf(g[e], win[k][e], dw[k][e]);
-                        acc[k][e] = fmaf(w[k][e], g[e], acc[k][e]);
+                            for (int e = 0; e < V; ++e) done[e] += v[e];
+                        }
+                        if (td >= 0) {
+                            float v[V];
+#pragma unroll
+                            for (int e = 0; e < V; ++e) v[e] = td < len ? done[e] : 0.f;
+                            store_row<T, V>((T*)p.dx + ((size_t)b * p.T + td) * p.C + c0, v);
+                        } else if (p.dstate) {
+                            store_row<T, V>((T*)p.dstate + ((size_t)b * (K - 1) + td + K - 1) * p.C + c0, done);
+                        }
                     }
                 }
-                // row t - (K-1) is complete
-                const int td = t - (K - 1);
-                const int from = td - (len - (K - 1));  // its place among the rows handed on as the window
-                if (p.dlast && from >= 0 && from < K - 1 && (td >= t0 || (t0 == 0 && td >= -(K - 1)))) {
-                    float v[V];
-                    load_row<T, V>(v, (const T*)p.dlast + ((size_t)b * (K - 1) + from) * p.C + c0, true);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) acc[0][e] += v[e];
-                }
-                if (td >= t0 && td < p.T) {
-                    if (td >= len) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) acc[0][e] = 0.f;
-                    }
-                    store_row<T, V>((T*)p.dx + ((size_t)b * p.T + td) * p.C + c0, acc[0]);
-                } else if (t0 == 0 && td < 0 && p.dstate) {
-                    store_row<T, V>((T*)p.dstate + ((size_t)b * (K - 1) + td + K - 1) * p.C + c0, acc[0]);
-                }
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) { win[k][e] = win[k + 1][e]; acc[k][e] = acc[k + 1][e]; }
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[K - 1][e] = 0.f;
             }
         }
     }
@@ -195,16 +222,14 @@ __global__ __launch_bounds__(256) void cconv_bwd_kernel(ga_causal_conv_bwd_param
 #pragma unroll
         for (int e = 0; e < V; ++e) red[threadIdx.x][e] = k < K ? dw[k < K ? k : 0][e] : db[e];
         __syncthreads();
-        if (ry == 0 && piece < m.pieces) {
+        if (ry == 0 && in) {
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = red[px][e];
             for (int j = 1; j < m.ry; ++j)
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[e] += red[j * m.px + px][e];
-            float* o = p.ws + ((size_t)part * (K + 1) + k) * p.C + c0;
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = v[e];
+            store_row<float, V>(p.ws + ((size_t)part * (K + 1) + k) * p.C + c0, v);
         }
     }
 }
@@ -247,7 +272,7 @@ int bad(int B, int T, int C, int K, int act, int dtype) {
     if (B < 1 || T < 1 || C < 1 || K < 1 || K > GA_CCONV_MAX_TAPS || (act != GA_ACT_NONE && act != GA_ACT_SILU)) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Map m = make_map(B, T, C, 1);
-    if ((m.runs + m.ry - 1) / m.ry * m.pb > 0x7fffffffL || (long)T + RUN + K > 0x7fffffffL) return GA_ERR_ARG;
+    if ((m.runs + m.ry - 1) / m.ry * m.pb > 0x7fffffffL || (long)T + 256 > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
 }
 
@@ -322,6 +347,7 @@ int ga_causal_conv_bwd(const ga_causal_conv_bwd_params* hp, int dtype, hipStream
     const int rc = bad(p.B, p.T, p.C, p.K, p.act, dtype);
     if (rc) return rc;
     if (!p.x || !p.w || !p.dy || !p.dx || !p.dw || !p.ws) return GA_ERR_ARG;
+    if ((uintptr_t)p.ws & 15) return GA_ERR_ALIGN;
     const int v = 4;
     const size_t bytes = v * (dtype == GA_DTYPE_BF16 ? 2 : 4);
     const bool vec = p.C % v == 0 && p.x_bs % v == 0 && p.x_ts % v == 0 && aligned(p.x, bytes) && aligned(p.dy, bytes) && aligned(p.dx, bytes) &&
