@@ -15,11 +15,11 @@ constexpr int MAX_PARTS = 1024;  // blocks of a backward launch at the most, eac
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 template <typename T, int V>
-__device__ __forceinline__ void stv(T* p, const float* v) {
+__device__ __forceinline__ void stv(T* p, unsigned col, const float* v) {
     Pack<T, V> r;
 #pragma unroll
     for (int e = 0; e < V; ++e) r.v[e] = (T)v[e];
-    *(Pack<T, V>*)p = r;
+    *(Pack<T, V>*)((char*)sq_scalar(p) + col * (unsigned)sizeof(T)) = r;
 }
 
 // sums of K values over the G threads of a row, in every one of them
@@ -48,16 +48,16 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[8][16], int
 
 #define BN_COLUMNS()                                                                  \
     const int tid = G == 64 ? threadIdx.x & 63 : threadIdx.x;                         \
-    const int w = G == 64 ? threadIdx.x >> 6 : 0;                                     \
+    const int w = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;     \
     constexpr int RPB = G == 64 ? 4 : 1;                                              \
     __shared__ __attribute__((aligned(16))) float red[2][8][16];                      \
     int slot = 0;                                                                     \
-    int col[P];                                                                       \
+    unsigned col[P];                                                                  \
     bool in[P];                                                                       \
     const float inv = 1.f / (float)p.C;                                               \
     _Pragma("unroll") for (int i = 0; i < P; ++i) {                                   \
-        col[i] = (i * G + tid) * V;                                                   \
-        in[i] = col[i] < p.C;                                                         \
+        col[i] = (unsigned)(i * G + tid) * V;                                         \
+        in[i] = col[i] < (unsigned)p.C;                                               \
         if (!in[i]) col[i] = 0; /* (read, never used or written) */                   \
     }
 
@@ -65,16 +65,19 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[8][16], int
 #define BN_ROWS _Pragma("unroll") for (int j = 0; j < R; ++j)
 
 template <int P, int V>
-__device__ __forceinline__ void load_cols(float (&o)[P][V], const float* p, const int (&col)[P], const bool (&in)[P], float none) {
+__device__ __forceinline__ void load_cols(float (&o)[P][V], const float* p, const unsigned (&col)[P], const bool (&in)[P], float none) {
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[i][e] = p && in[i] ? p[col[i] + e] : none;
+        for (int e = 0; e < V; ++e) {
+            const float v = p ? sq_scalar(p)[col[i] + e] : none;
+            o[i][e] = in[i] ? v : none;
+        }
 }
 template <typename T, int P, int V>
-__device__ __forceinline__ void load_raw(Pack<T, V> (&o)[P], const T* p, const int (&col)[P]) {
+__device__ __forceinline__ void load_raw(Pack<T, V> (&o)[P], const T* p, const unsigned (&col)[P]) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) o[i] = *(const Pack<T, V>*)(p + col[i]);
+    for (int i = 0; i < P; ++i) o[i] = *(const Pack<T, V>*)((const char*)sq_scalar(p) + col[i] * (unsigned)sizeof(T));
 }
 template <typename T, int P, int V>
 __device__ __forceinline__ void convert(float (&o)[P][V], const Pack<T, V> (&r)[P]) {
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_fwd_kernel(ga_block_n
                 if (k + j < rows_per_item) {
 #pragma unroll
                     for (int i = 0; i < P; ++i)
-                        if (in[i]) stv<TX, V>((TX*)p.r + off[j] + col[i], r[j][i]);
+                        if (in[i]) stv<TX, V>((TX*)p.r + off[j], col[i], r[j][i]);
                 }
             }
         }
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_fwd_kernel(ga_block_n
             BN_EACH r[j][i][e] = fmaf((r[j][i][e] - rm[j]) * rs[j], wv[i][e], bv[i][e]);
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i]) stv<TO, V>((TO*)p.y + off[j] + col[i], r[j][i]);
+                if (in[i]) stv<TO, V>((TO*)p.y + off[j], col[i], r[j][i]);
             if (p.stats && tid == 0) *(float4*)(p.stats + (row0 + k + j) * 4) = make_float4(om[j], os[j], rm[j], rs[j]);
         }
     }
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_bwd_kernel(ga_block_n
             if (p.dr) BN_EACH q[j][i][e] += in[i] && live[j] ? (float)dr[j][i].v[e] : 0.f;
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i] && live[j]) stv<TX, V>((TX*)p.dx + off[j] + col[i], q[j][i]);
+                if (in[i] && live[j]) stv<TX, V>((TX*)p.dx + off[j], col[i], q[j][i]);
         }
         if (p.branch) {
             BN_ROWS {
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_bwd_kernel(ga_block_n
                     }
 #pragma unroll
                     for (int i = 0; i < P; ++i)
-                        if (in[i] && live[j]) stv<TO, V>((TO*)p.dgate + off[j] + col[i], dg[i]);
+                        if (in[i] && live[j]) stv<TO, V>((TO*)p.dgate + off[j], col[i], dg[i]);
                 }
                 BN_EACH {
                     const float v = in[i] && live[j] ? q[j][i][e] : 0.f;
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_bwd_kernel(ga_block_n
                 BN_EACH q[j][i][e] = st[j].y * (fmaf(-o[j][i][e], a, q[j][i][e]) - b);
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (in[i] && live[j]) stv<TO, V>((TO*)p.dbranch + off[j] + col[i], q[j][i]);
+                    if (in[i] && live[j]) stv<TO, V>((TO*)p.dbranch + off[j], col[i], q[j][i]);
             }
         }
     }
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_bwd_kernel(ga_block_n
         if (w == 0) {
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (in[i]) stv<float, V>(out + (size_t)j * p.C + col[i], s[i]);
+                if (in[i]) stv<float, V>(out + (size_t)j * p.C, col[i], s[i]);
         }
     }
 }
@@ -435,13 +438,11 @@ int by_width(const A& p, bool vec, F f) {
         if (p.C <= 512) return f.template go<TX, TO, 64, 2, 4, F::R(2, 1)>(p);
         if (p.C <= 1024) return f.template go<TX, TO, 256, 1, 4, F::R(4, 2)>(p);
         if (p.C <= 2048) return f.template go<TX, TO, 256, 2, 4, F::R(2, 1)>(p);
-        if (p.C <= 4096) return f.template go<TX, TO, 1024, 1, 4, F::R(2, 1)>(p);
-        return f.template go<TX, TO, 1024, 2, 4, 1>(p);
+        return f.template go<TX, TO, 512, 2, 4, 1>(p);
     }
     if (p.C <= 256) return f.template go<TX, TO, 64, 4, 1, F::R(2, 1)>(p);
     if (p.C <= 1024) return f.template go<TX, TO, 256, 4, 1, F::R(2, 1)>(p);
-    if (p.C <= 4096) return f.template go<TX, TO, 1024, 4, 1, 1>(p);
-    return f.template go<TX, TO, 1024, 8, 1, 1>(p);
+    return f.template go<TX, TO, 512, 8, 1, 1>(p);
 }
 template <typename F, typename A>
 int by_type(const A& p, int xdt, int dt, bool vec, F f) {

@@ -301,15 +301,15 @@ int bwd(const ga_causal_conv_bwd_params& p, hipStream_t s) {
 }
 
 template <typename T, int V, typename P, typename F> int by_taps(const P& p, F f) {
-    switch (p.K) {
+    switch (p.K) {  // (window, gradients and weights of five taps and more for four channels do not fit the registers)
         case 1: return f.template go<T, V, 1>(p);
         case 2: return f.template go<T, V, 2>(p);
         case 3: return f.template go<T, V, 3>(p);
         case 4: return f.template go<T, V, 4>(p);
-        case 5: return f.template go<T, V, 5>(p);
-        case 6: return f.template go<T, V, 6>(p);
-        case 7: return f.template go<T, V, 7>(p);
-        case 8: return f.template go<T, V, 8>(p);
+        case 5: return f.template go<T, V == 4 ? 2 : V, 5>(p);
+        case 6: return f.template go<T, V == 4 ? 2 : V, 6>(p);
+        case 7: return f.template go<T, V == 4 ? 2 : V, 7>(p);
+        case 8: return f.template go<T, V == 4 ? 2 : V, 8>(p);
         default: return GA_ERR_ARG;
     }
 }
@@ -324,7 +324,7 @@ extern "C" {
 
 size_t ga_causal_conv_bwd_ws_elems(int B, int T, int C, int K) {
     if (bad(B, T, C, K, GA_ACT_NONE, GA_DTYPE_F32)) return 0;
-    const int one = parts_of(make_map(B, T, C, 1)), vec = parts_of(make_map(B, T, C, 4));
+    const int one = parts_of(make_map(B, T, C, 1)), vec = parts_of(make_map(B, T, C, K > 4 ? 2 : 4));
     return (size_t)(one > vec ? one : vec) * (K + 1) * C;
 }
 

@@ -6,7 +6,6 @@
 // a wave, and passes through LDS; B and C, which all channels of a group share, are first laid out in float32 in the order in which
 // the waves read them (scan_maps_kernel) and come in as scalar loads, so that they cost no vector instruction and no LDS bandwidth.
 #include "seq_common.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -15,6 +14,12 @@ constexpr int RPW = TS / 4;     // rows that one wave prepares and finishes
 constexpr int MAX_CHUNKS = 64;  // a block adds up the chunks before (behind) its own one by one
 
 typedef const __attribute__((address_space(4))) float* uniform_ptr;
+// `p` as a value that the compiler cannot trace: loads through it are issued where they stand, and not all at once at the top (their results
+// would be parked in vector registers, a move each way for every value)
+__device__ __forceinline__ uniform_ptr here(uniform_ptr p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
 
 struct Plan {
     int NS, NP;               // states of a wave, of the four waves
@@ -32,8 +37,7 @@ Plan make_plan(int B, int T, int C, int N, int G) {
     q.nCb = q.cbg * G;
     q.tiles = (T + TS - 1) / TS;
     const long blocks = (long)B * q.nCb;
-    static const long target = getenv("SCAN_BLOCKS") ? atol(getenv("SCAN_BLOCKS")) : 1024;
-    long want = (target + blocks - 1) / blocks;
+    long want = (1024 + blocks - 1) / blocks;  // four blocks a CU
     if (want > MAX_CHUNKS) want = MAX_CHUNKS;
     if (want > q.tiles) want = q.tiles;
     if (want < 1) want = 1;
@@ -72,9 +76,10 @@ __global__ __launch_bounds__(256) void scan_maps_kernel(const T* __restrict__ Bm
     }
 }
 
-// where a block and a lane are
+// Where a block and a lane are.  `d` counts channels, unsigned so that an address is a scalar base plus a 32-bit offset.
 struct Place {
-    int lane, w, chunk, b, g, d, len, tile0, tile1;
+    int lane, w, chunk, b, g, len, tile0, tile1;
+    unsigned d;
     bool ok;
     size_t item;  // first tile of the item's group in the maps
 };
@@ -88,40 +93,55 @@ __device__ __forceinline__ Place place(const Plan& q, int nch, int first_chunk, 
     x.g = cb / q.cbg;
     const int din = (cb % q.cbg) * 64 + x.lane;
     x.ok = din < q.Cg;
-    x.d = x.g * q.Cg + (x.ok ? din : q.Cg - 1);
+    x.d = (unsigned)(x.g * q.Cg + (x.ok ? din : q.Cg - 1));
     x.len = sq_len(lengths, x.b, T);
     x.tile0 = x.chunk * q.chunk_tiles;
     x.tile1 = min(x.tile0 + q.chunk_tiles, q.tiles);
     x.item = (size_t)(x.b * G + x.g) * q.tiles;
     return x;
 }
+template <typename T>
+__device__ __forceinline__ T& at(void* base, unsigned d) { return *(T*)((char*)sq_scalar(base) + d * (unsigned)sizeof(T)); }
+template <typename T>
+__device__ __forceinline__ T at(const void* base, unsigned d) { return *(const T*)((const char*)sq_scalar(base) + d * (unsigned)sizeof(T)); }
 
-// carry[s] <- exp(A sum of steps) carry[s] + end state, over the chunks from, from + dir, ... (count of them), eight loads in flight
-template <int NS>
-__device__ __forceinline__ void chain(float (&carry)[NS], const float (&A2)[NS], const float* ends, const float* ends_step, const Plan& q, int C, int b,
-                                      int w, int d, int from, int dir, int count) {
-    constexpr int U = NS <= 4 ? 8 : NS <= 8 ? 4 : 2;
+// A wave's rows of an activation, RPW of every tile from `row` on
+struct Rows {
+    const char* base;
+    int step;  // bytes from row to row
+    __device__ __forceinline__ Rows(const void* p, size_t elem, long bs, long ts, int b, int row)
+        : base((const char*)p + (b * bs + row * ts) * (long)elem), step((int)(ts * (long)elem)) {}
+    __device__ __forceinline__ void move(int tiles) { base += (long)tiles * TS * step; }
+    // row r of the wave's; `most`: T - 1 less the wave's first row (rows behind the last one read that one: no branch between the loads)
+    __device__ __forceinline__ const void* row(int r, int most) const { return base + (long)(min(r, most) * step); }
+};
+
+// carry[s] <- exp(A sum of steps) carry[s] + end of state n0 + s, over the chunks from, from + dir, ... (count of them), several loads in flight
+template <int K>
+__device__ __forceinline__ void chain(float (&carry)[K], const float (&A2)[K], const float* ends, const float* ends_step, const Plan& q, int C, int b,
+                                      int n0, unsigned d, int from, int dir, int count) {
+    constexpr int U = K <= 4 ? 8 : K <= 8 ? 4 : 2;
     for (int k = 0; k < count; k += U) {
-        float sum[U], end[U][NS];
+        float sum[U], end[U][K];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const size_t e = (size_t)b * q.chunks + (from + dir * min(k + i, count - 1));
-            sum[i] = ends_step[e * C + d];
+            sum[i] = at<float>(ends_step + e * C, d);
 #pragma unroll
-            for (int s = 0; s < NS; ++s) end[i][s] = ends[(e * q.NP + w * NS + s) * C + d];
+            for (int s = 0; s < K; ++s) end[i][s] = at<float>(ends + (e * q.NP + n0 + s) * C, d);
         }
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (k + i < count) {
 #pragma unroll
-                for (int s = 0; s < NS; ++s) carry[s] = fmaf(__builtin_amdgcn_exp2f(sum[i] * A2[s]), carry[s], end[i][s]);
+                for (int s = 0; s < K; ++s) carry[s] = fmaf(__builtin_amdgcn_exp2f(sum[i] * A2[s]), carry[s], end[i][s]);
             }
     }
 }
 
 // ENDS: only the state that each chunk but the last leaves behind when it starts from zero, and the sum of its steps
 // (the chunk's decay is exp(A * that sum)).  Otherwise the outputs, each chunk from the states of the chunks before it.
-template <typename T, int NS, bool ENDS>
+template <typename T, int NS, bool ENDS, bool HASZ>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     const ga_scan_params& p = a.p;
     const Plan& q = a.q;
@@ -130,7 +150,8 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     __shared__ float2 sd[TS][64];
     __shared__ float sy[ENDS ? 1 : 4][ENDS ? 1 : TS][64];
     const Place x = place(q, ENDS ? q.chunks - 1 : q.chunks, 0, p.G, p.T, p.lengths);
-    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
+    const int lane = x.lane, w = x.w, len = x.len;
+    const unsigned d = x.d;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
     float A2[NS], h[NS];
 #pragma unroll
@@ -140,25 +161,28 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
         h[s] = 0.f;
         if (!ENDS && p.state && n < p.N) h[s] = p.state[((size_t)x.b * p.C + d) * p.N + n];
     }
-    const T* up = (const T*)p.u + (size_t)x.b * p.u_bs;
-    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
-    const T* zp = ENDS || !p.z ? nullptr : (const T*)p.z + (size_t)x.b * p.z_bs;
+    const int row0 = x.tile0 * TS + w * RPW;
+    Rows us(p.u, sizeof(T), p.u_bs, p.u_ts, x.b, row0), ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0),
+        zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0);
+    char* yp = (char*)p.y + (((size_t)x.b * p.T + row0) * p.C) * sizeof(T);
+    const int ystep = p.C * (int)sizeof(T);
     T ru[RPW], rd[RPW], rz[RPW];
     float total = 0.f;
-    auto load = [&](int tile) __attribute__((always_inline)) {  // (rows behind the last one read that one: no branch between the loads)
+    auto load = [&](int tile) __attribute__((always_inline)) {
+        const int most = p.T - 1 - (tile * TS + w * RPW);
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            const int t = min(tile * TS + w * RPW + r, p.T - 1);
-            ru[r] = (up + (size_t)t * p.u_ts)[d];
-            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
-            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
+            ru[r] = at<T>(us.row(r, most), d);
+            rd[r] = at<T>(ds.row(r, most), d);
+            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
         }
     };
     load(x.tile0);
-    if (!ENDS) chain<NS>(h, A2, p.ends, p.ends_step, q, p.C, x.b, w, d, 0, 1, x.chunk);
+    if (!ENDS) chain<NS>(h, A2, p.ends, p.ends_step, q, p.C, x.b, w * NS, d, 0, 1, x.chunk);
     uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + x.tile0) * 4 + w) * (TS * 2 * NS));
     float m[2][U][2 * NS];
-    auto fetch = [&](float (&o)[U][2 * NS], uniform_ptr from) __attribute__((always_inline)) {
+    auto fetch = [&](float (&o)[U][2 * NS], uniform_ptr at) __attribute__((always_inline)) {
+        uniform_ptr from = here(at);
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -171,19 +195,22 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
             const int row = w * RPW + r, t = tile * TS + row;
             const bool live = x.ok && t < len;
             const float raw = (float)rd[r] + bias;
-            const float step = live ? p.softplus ? sq_softplus(raw) : raw : 0.f;
+            const float soft = sq_softplus(raw), step = live ? p.softplus ? soft : raw : 0.f;
             cu[r] = live ? (float)ru[r] : 0.f;
-            cz[r] = zp ? (float)rz[r] : 0.f;
+            cz[r] = HASZ ? (float)rz[r] : 0.f;
             total += step;
             sd[row][lane] = make_float2(step, step * cu[r]);
         }
         fetch(m[0], mp);
         __syncthreads();
-        if (tile + 1 < x.tile1) load(tile + 1);
+        if (tile + 1 < x.tile1) {
+            us.move(1), ds.move(1), zs.move(1);
+            load(tile + 1);
+        }
         if (!ENDS && p.hs && x.ok) {
             float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS) * p.C;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) (hp + (size_t)s * p.C)[d] = h[s];
+            for (int s = 0; s < NS; ++s) at<float>(hp + (size_t)s * p.C, d) = h[s];
         }
         float2 v[2][U];
         float y[TS];
@@ -222,9 +249,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
             for (int r = 0; r < RPW; ++r) {
                 const int row = w * RPW + r, t = tile * TS + row;
                 float o = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                if (zp) o *= sq_silu(cz[r]);
-                if (x.ok && t < p.T) ((T*)p.y + ((size_t)x.b * p.T + t) * p.C)[d] = (T)(t < len ? o : 0.f);
+                if (HASZ) o *= sq_silu(cz[r]);
+                if (x.ok && t < p.T) at<T>((void*)(yp + (long)(r * ystep)), d) = (T)(t < len ? o : 0.f);
             }
+            yp += (long)TS * ystep;
         }
     }
     if (ENDS) {
@@ -247,14 +275,15 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
 
 // The adjoint that each chunk but the first hands to the one before it when nothing comes in from behind:
 //   g_t = carry + C_t dyg_t, carry = exp(D_t A) g_t, from the chunk's last row to its first
-template <typename T, int NS>
+template <typename T, int NS, bool HASZ>
 __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int U = NS <= 4 ? 4 : NS <= 8 ? 2 : 1;
     __shared__ float2 sd[TS][64];
     const Place x = place(q, q.chunks - 1, 1, p.G, p.T, p.lengths);
-    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
+    const int lane = x.lane, w = x.w, len = x.len;
+    const unsigned d = x.d;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f;
     float A2[NS], c[NS];
 #pragma unroll
@@ -263,23 +292,24 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
         A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
         c[s] = 0.f;
     }
-    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
-    const T* zp = p.z ? (const T*)p.z + (size_t)x.b * p.z_bs : nullptr;
-    const T* gp = (const T*)p.dy + (size_t)x.b * p.T * p.C;
+    const int row0 = (x.tile1 - 1) * TS + w * RPW;
+    Rows ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0),
+        gs(p.dy, sizeof(T), (long)p.T * p.C, p.C, x.b, row0);
     T rd[RPW], rz[RPW], rg[RPW];
     float total = 0.f;
     auto load = [&](int tile) __attribute__((always_inline)) {
+        const int most = p.T - 1 - (tile * TS + w * RPW);
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            const int t = min(tile * TS + w * RPW + r, p.T - 1);
-            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
-            rg[r] = (gp + (size_t)t * p.C)[d];
-            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
+            rd[r] = at<T>(ds.row(r, most), d);
+            rg[r] = at<T>(gs.row(r, most), d);
+            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
         }
     };
     load(x.tile1 - 1);
     float m[2][U][NS];
-    auto fetch = [&](float (&o)[U][NS], uniform_ptr from) __attribute__((always_inline)) {
+    auto fetch = [&](float (&o)[U][NS], uniform_ptr at) __attribute__((always_inline)) {
+        uniform_ptr from = here(at);
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -292,15 +322,18 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
             const int row = w * RPW + r, t = tile * TS + row;
             const bool live = x.ok && t < len;
             const float raw = (float)rd[r] + bias;
-            const float step = live ? p.softplus ? sq_softplus(raw) : raw : 0.f;
+            const float soft = sq_softplus(raw), step = live ? p.softplus ? soft : raw : 0.f;
             float dy = (float)rg[r];
-            if (zp) dy *= sq_silu((float)rz[r]);
+            if (HASZ) dy *= sq_silu((float)rz[r]);
             total += step;
             sd[row][lane] = make_float2(step, live ? dy : 0.f);
         }
         fetch(m[0], mp + (TS - U) * 2 * NS);
         __syncthreads();
-        if (tile > x.tile0) load(tile - 1);
+        if (tile > x.tile0) {
+            ds.move(-1), zs.move(-1), gs.move(-1);
+            load(tile - 1);
+        }
         float2 v[2][U];
 #pragma unroll
         for (int i = 0; i < U; ++i) v[0][i] = sd[TS - U + i][lane];
@@ -333,80 +366,136 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
 }
 
 // Per tile, from the last to the first: the states again from the one saved at the tile's start (kept in registers, with the decays), then
-// the adjoint backwards through them; NB states of a wave at a time.
-template <typename T, int NS>
+// the adjoint backwards through them; NB states of a wave at a time.  With more than NB the adjoint, dA and the rows' values wait in LDS for their turn: a
+// vector register spilled here is not only slow (the compiler has been seen to place such copies under a branch's mask).
+template <typename T, int NS, bool HASZ>
 __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
-    constexpr int NB = NS < 4 ? NS : 4, U = 2;
+    constexpr int NB = NS < 4 ? NS : 4, SB = NS / NB, U = 2;
     __shared__ float2 sd[TS][64];     // step, step * u
     __shared__ float sg[TS][64];      // dy * gate
     __shared__ float sy[4][TS][64];   // <C, h> over a wave's states
     __shared__ float2 ss[4][TS][64];  // <g, B>, <g a h_prev, A>
     __shared__ float sm[4][TS][2 * NS];
+    __shared__ float wait[SB > 1 ? 2 * NS + 7 * RPW : 1][SB > 1 ? 256 : 1];
     const Place x = place(q, q.chunks, 0, p.G, p.T, p.lengths);
-    const int lane = x.lane, w = x.w, d = x.d, len = x.len;
+    const int lane = x.lane, w = x.w, len = x.len;
+    const unsigned d = x.d;
     const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
-    float A2[NS], c[NS], dA[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-        const int n = w * NS + s;
-        A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
-        c[s] = p.dlast && n < p.N && x.ok ? p.dlast[((size_t)x.b * p.C + d) * p.N + n] : 0.f;
-        dA[s] = 0.f;
-    }
-    const T* up = (const T*)p.u + (size_t)x.b * p.u_bs;
-    const T* dp = (const T*)p.delta + (size_t)x.b * p.delta_bs;
-    const T* zp = p.z ? (const T*)p.z + (size_t)x.b * p.z_bs : nullptr;
-    const size_t orow = (size_t)x.b * p.T * p.C;
-    const T* gp = (const T*)p.dy + orow;
+    const int row0 = (x.tile1 - 1) * TS + w * RPW;
+    Rows us(p.u, sizeof(T), p.u_bs, p.u_ts, x.b, row0), ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0),
+        zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0), gs(p.dy, sizeof(T), (long)p.T * p.C, p.C, x.b, row0);
+    size_t orow = ((size_t)x.b * p.T + row0) * p.C * sizeof(T);  // of the outputs, in bytes
+    const int ostep = p.C * (int)sizeof(T);
     T ru[RPW], rd[RPW], rz[RPW], rg[RPW];
+    float hn[NB];
+    auto load_h = [&](int tile, int sb) __attribute__((always_inline)) {
+        const float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS + sb * NB) * p.C;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) hn[j] = at<float>(hp + (size_t)j * p.C, d);
+    };
     auto load = [&](int tile) __attribute__((always_inline)) {
+        load_h(tile, 0);
+        const int most = p.T - 1 - (tile * TS + w * RPW);
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            const int t = min(tile * TS + w * RPW + r, p.T - 1);
-            ru[r] = (up + (size_t)t * p.u_ts)[d];
-            rd[r] = (dp + (size_t)t * p.delta_ts)[d];
-            rg[r] = (gp + (size_t)t * p.C)[d];
-            if (zp) rz[r] = (zp + (size_t)t * p.z_ts)[d];
+            ru[r] = at<T>(us.row(r, most), d);
+            rd[r] = at<T>(ds.row(r, most), d);
+            rg[r] = at<T>(gs.row(r, most), d);
+            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
         }
     };
-    load(x.tile1 - 1);
-    chain<NS>(c, A2, p.ends, p.ends_step, q, p.C, x.b, w, d, q.chunks - 1, -1, q.chunks - 1 - x.chunk);
+    if (SB == 1) load(x.tile1 - 1);
+    float A2[NB], c[NB], dA[NB];
+    auto load_A = [&](int sb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = w * NS + sb * NB + j;
+            const float v = p.A[(size_t)d * p.N + min(n, p.N - 1)] * SQ_LOG2E;
+            A2[j] = n < p.N ? v : 0.f;
+        }
+    };
+#pragma unroll
+    for (int sb = 0; sb < SB; ++sb) {
+        load_A(sb);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = w * NS + sb * NB + j;
+            c[j] = p.dlast && n < p.N && x.ok ? p.dlast[((size_t)x.b * p.C + d) * p.N + n] : 0.f;
+            dA[j] = 0.f;
+        }
+        chain<NB>(c, A2, p.ends, p.ends_step, q, p.C, x.b, w * NS + sb * NB, d, q.chunks - 1, -1, q.chunks - 1 - x.chunk);
+        if (SB > 1) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                wait[sb * NB + j][threadIdx.x] = c[j];
+                wait[NS + sb * NB + j][threadIdx.x] = 0.f;
+            }
+        }
+    }
     float dD = 0.f, dbias = 0.f;
+    // what only a tile's end needs is read again from the kernel's arguments there: kept over the loop it costs the scalar registers of B and C
+    const __attribute__((address_space(4))) BwdArgs* args = (const __attribute__((address_space(4))) BwdArgs*)__builtin_amdgcn_kernarg_segment_ptr();
     for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
-        const float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS) * p.C;
-        float cu[RPW], craw[RPW], cz[RPW], cdy[RPW], cstep[RPW], cg[RPW], h0[NS];
-#pragma unroll
-        for (int s = 0; s < NS; ++s) h0[s] = (hp + (size_t)s * p.C)[d];
+        float cu[RPW], cslope[RPW], cz[RPW], csig[RPW], cdy[RPW], cstep[RPW], cg[RPW], h0[NB];
+        if (SB > 1) load(tile);
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
             const bool live = x.ok && t < len;
-            craw[r] = (float)rd[r] + bias;
-            cstep[r] = live ? p.softplus ? sq_softplus(craw[r]) : craw[r] : 0.f;
+            const float raw = (float)rd[r] + bias;
+            float slope;
+            const float soft = sq_softplus(raw, slope), step = p.softplus ? soft : raw;
+            cslope[r] = p.softplus ? slope : 1.f;
+            cstep[r] = live ? step : 0.f;
             cu[r] = live ? (float)ru[r] : 0.f;
             cdy[r] = live ? (float)rg[r] : 0.f;
-            cz[r] = zp && live ? (float)rz[r] : 0.f;
-            cg[r] = zp ? cdy[r] * sq_silu(cz[r]) : cdy[r];
+            cz[r] = HASZ && live ? (float)rz[r] : 0.f;
+            csig[r] = HASZ ? sq_sigmoid(cz[r]) : 1.f;
+            cg[r] = HASZ ? cdy[r] * (cz[r] * csig[r]) : cdy[r];
             sd[row][lane] = make_float2(cstep[r], cstep[r] * cu[r]);
             sg[row][lane] = cg[r];
         }
-        __syncthreads();
-        if (tile > x.tile0) load(tile - 1);
+        if (SB == 1) {
 #pragma unroll
-        for (int sb = 0; sb < NS / NB; ++sb) {
+            for (int j = 0; j < NB; ++j) h0[j] = hn[j];
+        } else {
+#pragma unroll
+            for (int r = 0; r < RPW; ++r) {
+                float* keep = &wait[2 * NS + 7 * r][threadIdx.x];
+                keep[0] = cu[r], keep[256] = cslope[r], keep[512] = cz[r], keep[768] = csig[r], keep[1024] = cdy[r], keep[1280] = cstep[r], keep[1536] = cg[r];
+            }
+        }
+        __syncthreads();
+        if (tile > x.tile0) {
+            us.move(-1), ds.move(-1), zs.move(-1), gs.move(-1);
+            if (SB == 1) load(tile - 1);  // (with more states there is no room for rows on their way)
+        }
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb) {
+            if (SB > 1) {
+                load_A(sb);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    h0[j] = hn[j];
+                    c[j] = wait[sb * NB + j][threadIdx.x];
+                    dA[j] = wait[NS + sb * NB + j][threadIdx.x];
+                }
+                if (sb + 1 < SB) load_h(tile, sb + 1);
+            }
             float h[TS][NB], av[TS][NB];
             float m[2][U][2 * NB];
             float2 v[2][U];
             auto fetch = [&](int set, int t0) __attribute__((always_inline)) {
+                uniform_ptr from = here(mp + t0 * 2 * NS + sb * NB);
 #pragma unroll
                 for (int i = 0; i < U; ++i) {
 #pragma unroll
                     for (int j = 0; j < NB; ++j) {
-                        m[set][i][j] = mp[(t0 + i) * 2 * NS + sb * NB + j];
-                        m[set][i][NB + j] = mp[(t0 + i) * 2 * NS + NS + sb * NB + j];
+                        m[set][i][j] = from[i * 2 * NS + j];
+                        m[set][i][NB + j] = from[i * 2 * NS + NS + j];
                     }
                     v[set][i] = sd[t0 + i][lane];
                 }
@@ -421,14 +510,14 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                     const int t = k * U + i;
                     const float2 o = v[k & 1][i];
                     const float* mm = m[k & 1][i];
-                    float y = sb && zp ? sy[w][t][lane] : 0.f;
+                    float y = sb && HASZ ? sy[w][t][lane] : 0.f;
 #pragma unroll
                     for (int j = 0; j < NB; ++j) {
-                        av[t][j] = __builtin_amdgcn_exp2f(o.x * A2[sb * NB + j]);
-                        h[t][j] = fmaf(av[t][j], t ? h[t - 1][j] : h0[sb * NB + j], o.y * mm[j]);
+                        av[t][j] = __builtin_amdgcn_exp2f(o.x * A2[j]);
+                        h[t][j] = fmaf(av[t][j], t ? h[t - 1][j] : h0[j], o.y * mm[j]);
                         y = fmaf(mm[NB + j], h[t][j], y);
                     }
-                    if (zp) sy[w][t][lane] = y;
+                    if (HASZ) sy[w][t][lane] = y;
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -439,7 +528,9 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                 for (int i = 0; i < U; ++i) gy[set][i] = sg[t0 + i][lane];
             };
             fetch_back(0, TS - U);
-            constexpr int PER = 64 / (2 * NB);  // lanes that share a value after the first folds
+            // a row's 2 NB products are folded until a lane has one, summed over 2 NB lanes; KEEP rows of these then over the other lanes
+            constexpr int KEEP = TS < 64 / (2 * NB) ? TS : 64 / (2 * NB);
+            float part[KEEP];
 #pragma unroll
             for (int k = 0; k < TS / U; ++k) {
                 if (k + 1 < TS / U) fetch_back((k + 1) & 1, TS - (k + 2) * U);
@@ -454,64 +545,88 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                     float val[2 * NB];
 #pragma unroll
                     for (int j = 0; j < NB; ++j) {
-                        const int s = sb * NB + j;
-                        const float gv = fmaf(mm[NB + j], dy, c[s]);
+                        const float gv = fmaf(mm[NB + j], dy, c[j]);
                         val[j] = gv * o.y;
                         val[NB + j] = dy * h[t][j];
                         s12.x = fmaf(gv, mm[j], s12.x);
-                        c[s] = av[t][j] * gv;
-                        const float qv = c[s] * (t ? h[t - 1][j] : h0[s]);
-                        s12.y = fmaf(qv, A2[s], s12.y);
-                        dA[s] = fmaf(qv, o.x, dA[s]);
+                        c[j] = av[t][j] * gv;
+                        const float qv = c[j] * (t ? h[t - 1][j] : h0[j]);
+                        s12.y = fmaf(qv, A2[j], s12.y);
+                        dA[j] = fmaf(qv, o.x, dA[j]);
                     }
                     ss[w][t][lane] = s12;
-                    const float sum = sq_lane_sums<2 * NB>(val, lane);
-                    if (lane % PER == 0) {
-                        const int i2 = lane / PER;  // B's share in the first NB, C's in the others
-                        sm[w][t][(i2 / NB) * NS + sb * NB + i2 % NB] = sum;
+                    part[t % KEEP] = sq_fold_down<2 * NB, 32>(val, lane);
+                    if (t % KEEP == 0) {
+                        constexpr int PER = 64 / (2 * NB), EXTRA = PER / KEEP;
+                        static_assert(EXTRA <= 2, "at most one lane bit is left");
+                        float sum = sq_fold_down<KEEP, PER / 2>(part, lane);
+                        if (EXTRA == 2) sum += sq_dpp<0xB1>(sum);
+                        const int i2 = lane / PER, row = t + lane % PER / EXTRA;  // B's share in the first NB, C's in the others
+                        sm[w][row][(i2 / NB) * NS + sb * NB + i2 % NB] = sum;     // (EXTRA lanes write the same sum)
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (SB > 1) {
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    wait[sb * NB + j][threadIdx.x] = c[j];
+                    wait[NS + sb * NB + j][threadIdx.x] = dA[j];
+                }
+            }
         }
         __syncthreads();
+        asm volatile("" : "+s"(args));
+        const auto& pc = args->p;
+        if (SB > 1) {
+#pragma unroll
+            for (int r = 0; r < RPW; ++r) {
+                const float* keep = &wait[2 * NS + 7 * r][threadIdx.x];
+                cu[r] = keep[0], cslope[r] = keep[256], cz[r] = keep[512], csig[r] = keep[768], cdy[r] = keep[1024], cstep[r] = keep[1280], cg[r] = keep[1536];
+            }
+        }
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
             const int row = w * RPW + r, t = tile * TS + row;
             const bool live = x.ok && t < len;
             const float2 x0 = ss[0][row][lane], x1 = ss[1][row][lane], x2 = ss[2][row][lane], x3 = ss[3][row][lane];
             const float s1 = (x0.x + x1.x) + (x2.x + x3.x), s2 = ((x0.y + x1.y) + (x2.y + x3.y)) * SQ_LN2;
-            const float du = fmaf(cstep[r], s1, Dd * cg[r]);
-            float dd = fmaf(cu[r], s1, s2);
-            if (p.softplus) dd *= sq_sigmoid(craw[r]);
-            dd = live ? dd : 0.f;
+            const float du = fmaf(cstep[r], s1, Dd * cg[r]), dd = live ? fmaf(cu[r], s1, s2) * cslope[r] : 0.f;
             dD = fmaf(cg[r], cu[r], dD);
             dbias += dd;
-            if (x.ok && t < p.T) {
-                const size_t o = orow + (size_t)t * p.C;
-                ((T*)p.du + o)[d] = (T)(live ? du : 0.f);
-                ((T*)p.ddelta + o)[d] = (T)dd;
-                if (zp) {
-                    const float y = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                    ((T*)p.dz + o)[d] = (T)(live ? cdy[r] * y * sq_silu_slope(cz[r]) : 0.f);
-                }
+            float dz = 0.f;
+            if (HASZ) {
+                const float y = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
+                dz = cdy[r] * y * csig[r] * fmaf(cz[r], 1.f - csig[r], 1.f);
+            }
+            if (t < p.T && x.ok) {
+                const size_t o = orow + (long)(r * ostep);
+                at<T>((void*)((char*)pc.du + o), d) = (T)(live ? du : 0.f);
+                at<T>((void*)((char*)pc.ddelta + o), d) = (T)dd;
+                if (HASZ) at<T>((void*)((char*)pc.dz + o), d) = (T)(live ? dz : 0.f);
             }
         }
+        orow -= (long)TS * ostep;
         // this block's share of dB and dC, in the layout of the maps
         const int slab = (blockIdx.x % q.nCb) % q.cbg;
-        float* mo = p.dmaps + ((size_t)slab * p.B * p.G * q.tiles + x.item + tile) * (4 * TS * 2 * NS);
-        for (int i = threadIdx.x; i < 4 * TS * 2 * NS; i += 256) mo[i] = (&sm[0][0][0])[i];
+        float* mo = pc.dmaps + ((size_t)slab * pc.B * pc.G * q.tiles + x.item + tile) * (4 * TS * 2 * NS);
+#pragma unroll
+        for (int i = 0; i < (4 * TS * 2 * NS + 255) / 256; ++i) {
+            const int k = i * 256 + threadIdx.x;
+            if (4 * TS * 2 * NS % 256 == 0 || k < 4 * TS * 2 * NS) at<float>(mo, (unsigned)k) = (&sm[0][0][0])[k];
+        }
         __syncthreads();
     }
     const size_t e = (size_t)x.b * q.chunks + x.chunk;
-    if (x.ok) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) p.dparams[(e * (q.NP + 2) + w * NS + s) * p.C + d] = dA[s];
-        if (p.dstate && x.chunk == 0) {
+    for (int sb = 0; sb < SB; ++sb) {
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int n = w * NS + s;
-                if (n < p.N) p.dstate[((size_t)x.b * p.C + d) * p.N + n] = c[s];
+        for (int j = 0; j < NB; ++j) {
+            const int s = sb * NB + j, n = w * NS + s;
+            const float dAv = SB > 1 ? wait[NS + s][threadIdx.x] : dA[j], cv = SB > 1 ? wait[s][threadIdx.x] : c[j];
+            if (x.ok) {
+                p.dparams[(e * (q.NP + 2) + n) * p.C + d] = dAv;
+                if (p.dstate && x.chunk == 0 && n < p.N) p.dstate[((size_t)x.b * p.C + d) * p.N + n] = cv;
             }
         }
     }
@@ -605,11 +720,15 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, i
 }
 
 int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
-    if (B < 1 || T < 1 || C < 1 || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
+    if (B < 1 || T < 1 || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
     if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
+}
+
+bool bad_strides(long a, long b, long c) {
+    return a < 0 || b < 0 || c < 0 || a > GA_SCAN_MAX_STRIDE || b > GA_SCAN_MAX_STRIDE || c > GA_SCAN_MAX_STRIDE;
 }
 
 int grid_for(size_t n) {
@@ -621,24 +740,29 @@ template <typename T, int NS>
 int launch_fwd(const Args& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_fwd_kernel<T, NS, true><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_fwd_kernel<T, NS, true, false><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    scan_fwd_kernel<T, NS, false><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    if (a.p.z) scan_fwd_kernel<T, NS, false, true><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    else scan_fwd_kernel<T, NS, false, false><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
 
-template <typename T, int NS>
-int launch_bwd(const BwdArgs& a, hipStream_t s) {
+template <typename T, int NS, bool HASZ>
+int launch_bwd_z(const BwdArgs& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_bwd_ends_kernel<T, NS><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_bwd_ends_kernel<T, NS, HASZ><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    scan_bwd_kernel<T, NS><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    scan_bwd_kernel<T, NS, HASZ><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
+}
+template <typename T, int NS>
+int launch_bwd(const BwdArgs& a, hipStream_t s) {
+    return a.p.z ? launch_bwd_z<T, NS, true>(a, s) : launch_bwd_z<T, NS, false>(a, s);
 }
 
 #define SCAN_DISPATCH(FN, T, ARGS)                 \
@@ -693,6 +817,7 @@ int ga_scan_fwd(const ga_scan_params* hp, int dtype, hipStream_t s) {
     if (rc) return rc;
     const Args a{p, make_plan(p.B, p.T, p.C, p.N, p.G)};
     if (!p.u || !p.delta || !p.A || !p.Bm || !p.Cm || !p.y || !p.maps || (a.q.chunks > 1 && (!p.ends || !p.ends_step))) return GA_ERR_ARG;
+    if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
     return dtype == GA_DTYPE_BF16 ? fwd<bf16_t>(a, s) : fwd<float>(a, s);
 }
@@ -706,6 +831,7 @@ int ga_scan_bwd(const ga_scan_bwd_params* hp, int dtype, hipStream_t s) {
     if (!p.u || !p.delta || !p.A || !p.dy || !p.maps || !p.hs || !p.du || !p.ddelta || !p.dA || !p.dBm || !p.dCm || !p.dmaps || !p.dparams ||
         (!p.z) != (!p.dz) || (a.q.chunks > 1 && (!p.ends || !p.ends_step)))
         return GA_ERR_ARG;
+    if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
     return dtype == GA_DTYPE_BF16 ? bwd<bf16_t>(a, s) : bwd<float>(a, s);
 }

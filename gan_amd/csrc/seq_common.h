@@ -4,14 +4,6 @@
 
 constexpr float SQ_LOG2E = 1.4426950408889634f, SQ_LN2 = 0.6931471805599453f;
 
-// exp(x) for x <= 0 to about an ulp: x * log2(e) as a rounded product plus its rounding error (without the second term the relative error is
-// |x| * 2^-24: 4e-7 at the softplus arguments of small step sizes)
-__device__ __forceinline__ float sq_exp(float x) {
-    const float t = x * SQ_LOG2E;
-    const float lo = fmaf(x, SQ_LOG2E, -t) + x * 1.925963033500e-8f;  // log2(e) - fp32(log2(e))
-    const float e = __builtin_amdgcn_exp2f(t);
-    return x < -100.f ? e : fmaf(e, lo * SQ_LN2, e);
-}
 __device__ __forceinline__ float sq_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * SQ_LOG2E)); }
 __device__ __forceinline__ float sq_silu(float x) { return x * sq_sigmoid(x); }
 // d silu(x) / dx
@@ -19,12 +11,29 @@ __device__ __forceinline__ float sq_silu_slope(float x) {
     const float s = sq_sigmoid(x);
     return s * fmaf(x, 1.f - s, 1.f);
 }
-// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|); log1p(e) = log(w) + (e - (w - 1)) / w with w = fl(1 + e): the second term gives
-// back what the sum lost, so that small results keep all their digits
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|).  e: exp2 of the rounded product t = -|x| log2(e), times 1 + r with r = what t lacks
+// (without it e is off by |x| 2^-24 of itself: 4e-7 at the arguments of small step sizes).  log1p(e) = log(w) + (e - (w - 1)) / w with
+// w = fl(1 + e): the second term gives back what the sum lost, so that small results keep all their digits.  max(x, 0) as (x + |x|) / 2, which
+// passes a NaN on.  `sigmoid`: the slope, 1 / (1 + exp(-x)), from the same e and w.
+__device__ __forceinline__ float sq_softplus(float x, float& sigmoid) {
+    const float ax = fminf(fabsf(x), 100.f), t = -ax * SQ_LOG2E;
+    const float r = fmaf(-t, -1.9046542e-9f, fmaf(-t, SQ_LN2, -ax));  // ln 2 = fp32(ln 2) - 1.9046542e-9
+    const float e2 = __builtin_amdgcn_exp2f(t), e = fmaf(e2, r, e2), w = 1.f + e, rw = __builtin_amdgcn_rcpf(w);
+    sigmoid = (x < 0.f ? e : 1.f) * rw;
+    return fmaf(0.5f, x + fabsf(x), fmaf(__builtin_amdgcn_logf(w), SQ_LN2, (e - (w - 1.f)) * rw));
+}
 __device__ __forceinline__ float sq_softplus(float x) {
-    const float e = sq_exp(-fabsf(x)), w = 1.f + e;
-    const float l = fmaf(__builtin_amdgcn_logf(w), SQ_LN2, (e - (w - 1.f)) * __builtin_amdgcn_rcpf(w));
-    return (x > 0.f ? x : x != x ? x : 0.f) + l;
+    float s;
+    return sq_softplus(x, s);
+}
+
+// A pointer that is the same in all lanes, as a scalar that is added to nowhere else: base plus a 32-bit offset per lane is then the address of a
+// load (otherwise the compiler folds the offset into a 64-bit vector add, and two registers, for every row).
+template <typename P>
+__device__ __forceinline__ P* sq_scalar(P* p) {
+    const uint64_t u = (uint64_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+    return (P*)(((uint64_t)hi << 32) | lo);
 }
 
 __device__ __forceinline__ int sq_len(const int* lengths, int b, int T) {
@@ -51,24 +60,52 @@ template <int CTRL>
 __device__ __forceinline__ float sq_fold(float a, float b, bool up) {
     return (up ? b : a) + sq_dpp<CTRL>(up ? a : b);
 }
-// n values (a power of two) in v; lane l leaves with v[0] = the sum of value (the top log2 n bits of l)
+// V values (a power of two) in v, folded over the lane bits TOP, TOP / 2, ... until one is left: a lane leaves with the sum, over the lanes that
+// differ from it in these bits, of the value that they number
+template <int V, int TOP>
+__device__ __forceinline__ float sq_fold_down(float (&v)[V], int lane) {
+    static_assert(V >= 1 && (V & (V - 1)) == 0 && V <= 2 * TOP, "a power of two, and a lane bit for each halving");
+    int n = V;
+    if (TOP >= 32 && n > 1) {
+        n >>= 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = sq_fold32(v[i], v[i + n]);
+    }
+    if (TOP >= 16 && n > 1) {
+        n >>= 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = sq_fold16(v[i], v[i + n]);
+    }
+    if (TOP >= 8 && n > 1) {
+        n >>= 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = sq_fold<0x128>(v[i], v[i + n], lane & 8);  // rotate by 8 within 16
+    }
+    if (TOP >= 4 && n > 1) {
+        n >>= 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = sq_fold<0x141>(v[i], v[i + n], lane & 4);  // mirror within 8
+    }
+    if (TOP >= 2 && n > 1) {
+        n >>= 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = sq_fold<0x4E>(v[i], v[i + n], lane & 2);  // quads: 2 3 0 1
+    }
+    if (TOP >= 1 && n > 1) v[0] = sq_fold<0xB1>(v[0], v[1], lane & 1);  // quads: 1 0 3 2
+    return v[0];
+}
+// V values, each summed over all 64 lanes: lane l leaves with the sum of value (the top log2 V bits of l)
 template <int V>
 __device__ __forceinline__ float sq_lane_sums(float (&v)[V], int lane) {
-    static_assert(V >= 1 && V <= 64 && (V & (V - 1)) == 0, "a power of two");
-    int n = V;
-#define SQ_FOLD(FN, ...)                                                              \
-    if (n > 1) {                                                                      \
-        n >>= 1;                                                                      \
-        _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = FN(v[i], v[i + n] __VA_ARGS__); \
-    } else
-    SQ_FOLD(sq_fold32) v[0] = sq_fold32(v[0], v[0]);
-    SQ_FOLD(sq_fold16) v[0] = sq_fold16(v[0], v[0]);
-    SQ_FOLD(sq_fold<0x128>, , lane & 8) v[0] += sq_dpp<0x128>(v[0]);  // rotate by 8 within 16
-    SQ_FOLD(sq_fold<0x141>, , lane & 4) v[0] += sq_dpp<0x141>(v[0]);  // mirror within 8
-    SQ_FOLD(sq_fold<0x4E>, , lane & 2) v[0] += sq_dpp<0x4E>(v[0]);    // quads: 2 3 0 1
-    SQ_FOLD(sq_fold<0xB1>, , lane & 1) v[0] += sq_dpp<0xB1>(v[0]);    // quads: 1 0 3 2
-#undef SQ_FOLD
-    return v[0];
+    float s = sq_fold_down<V, 32>(v, lane);
+    constexpr int REST = 64 / V;
+    if (REST >= 64) s = sq_fold32(s, s);
+    if (REST >= 32) s = sq_fold16(s, s);
+    if (REST >= 16) s += sq_dpp<0x128>(s);
+    if (REST >= 8) s += sq_dpp<0x141>(s);
+    if (REST >= 4) s += sq_dpp<0x4E>(s);
+    if (REST >= 2) s += sq_dpp<0xB1>(s);
+    return s;
 }
 
 // One column of a [rows][cols] matrix of partial sums, added up by `groups` threads of a block (thread group w of the column) in double: eight

@@ -560,6 +560,7 @@ int ga_causal_conv_step(const ga_causal_conv_step_params* h_params, int dtype, g
  * fp32 (the last two may be NULL); state [B][C][N] fp32 (NULL: zero); last [B][C][N] (may be NULL) receives the state at the item's end.
  * maps / hs / ends / ends_step: fp32 buffers of ga_scan_sizes() elements; maps and hs are what the backward pass reads (hs NULL: not wanted). */
 #define GA_SCAN_MAX_STATES 64
+#define GA_SCAN_MAX_STRIDE (1 << 24) /* elements from a row to the next, and channels, at the most */
 typedef struct ga_scan_buffers {
     size_t maps;      /* B and C in float32, in the kernels' order */
     size_t hs;        /* the state at every 16th row */
@@ -606,7 +607,7 @@ int ga_scan_step(const ga_scan_step_params* h_params, int dtype, ga_stream_t str
  * and a gate per row in dtype (xdtype = dtype, or fp32 with bf16).  w, b, wp, bp, scale [C] fp32, each may be NULL (1, 0, 1, 0, 1);
  * gate: NULL, fp32 [B][C] (gate_rows = 0) or dtype [B][T][C] (gate_rows = 1); ab: NULL or fp32 [B][2C] = (a | s).  branch NULL: r is x, not
  * written.  stats [B*T][4] fp32 or NULL: means and reciprocal deviations of the two norms for the backward pass. */
-#define GA_BNORM_MAX_C 8192
+#define GA_BNORM_MAX_C 4096
 typedef struct ga_block_norm_params {
     const void* x; const void* branch; const void* gate;
     const float* w; const float* b; const float* wp; const float* bp; const float* scale; const float* ab;

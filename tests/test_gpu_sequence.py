@@ -271,7 +271,7 @@ NORM = [  # B, T, C, x type, dtype, layer, post, gate, scale, ab, affine
     (2, 3, 1028, F32, BF, False, True, "row", True, False, True),
     (2, 2, 2049, F32, F32, True, True, "item", True, True, True),
     (1, 3, 4096, F32, BF, False, True, None, True, False, True),
-    (1, 2, 8192, BF, BF, True, True, "row", True, True, True),
+    (1, 2, 4093, BF, BF, True, True, "row", True, True, True),
     (300, 1, 64, BF, BF, False, True, "item", True, True, True),
     (2, 700, 36, F32, F32, False, True, "row", True, False, True),
     (4, 6, 48, F32, BF, False, None, None, False, True, True),     # no branch
