@@ -30,7 +30,7 @@ struct Plan {
 
 Plan make_plan(int B, int T, int C, int N, int G) {
     Plan q;
-    q.NS = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
+    q.NS = N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
     q.NP = 4 * q.NS;
     q.Cg = C / G;
     q.cbg = (q.Cg + 63) / 64;
@@ -49,10 +49,12 @@ Plan make_plan(int B, int T, int C, int N, int G) {
 struct Args {
     ga_scan_params p;
     Plan q;
+    int vec;  // quads of channels can be read and written at once
 };
 struct BwdArgs {
     ga_scan_bwd_params p;
     Plan q;
+    int vec;
 };
 
 // maps[b][group][tile][wave][row][B: NS | C: NS] in float32, wave w holding the states w NS .. w NS + NS - 1; zero rows behind an item's length and
@@ -105,16 +107,113 @@ __device__ __forceinline__ T& at(void* base, unsigned d) { return *(T*)((char*)s
 template <typename T>
 __device__ __forceinline__ T at(const void* base, unsigned d) { return *(const T*)((const char*)sq_scalar(base) + d * (unsigned)sizeof(T)); }
 
-// A wave's rows of an activation, RPW of every tile from `row` on
-struct Rows {
-    const char* base;
-    int step;  // bytes from row to row
-    __device__ __forceinline__ Rows(const void* p, size_t elem, long bs, long ts, int b, int row)
-        : base((const char*)p + (b * bs + row * ts) * (long)elem), step((int)(ts * (long)elem)) {}
-    __device__ __forceinline__ void move(int tiles) { base += (long)tiles * TS * step; }
-    // row r of the wave's; `most`: T - 1 less the wave's first row (rows behind the last one read that one: no branch between the loads)
-    __device__ __forceinline__ const void* row(int r, int most) const { return base + (long)(min(r, most) * step); }
+template <typename T> struct alignas(4 * sizeof(T)) Quad { T v[4]; };
+
+// The four elements of a tile that a lane prepares and finishes.  VEC: four adjacent channels of one row, one access for all four rows of a wave;
+// otherwise (alignment, odd widths) one channel of each of the four rows.
+template <bool VEC>
+struct Elems {
+    int lane, w, g, first, Cg;  // first: the block's first channel in its group
+    __device__ __forceinline__ Elems(const Place& x, const Plan& q)
+        : lane(x.lane), w(x.w), g(x.g), first((int)(blockIdx.x % q.nCb) % q.cbg * 64), Cg(q.Cg) {}
+    __device__ __forceinline__ int row(int e) const { return w * RPW + (VEC ? lane >> 4 : e); }
+    __device__ __forceinline__ int ch(int e) const { return VEC ? (lane & 15) * 4 + e : lane; }
+    __device__ __forceinline__ bool ok() const { return first + ch(0) < Cg; }  // (VEC: groups of whole quads only)
+    __device__ __forceinline__ unsigned d(int e) const {
+        const int c = first + ch(0);
+        return (unsigned)(g * Cg + (ok() ? c : Cg - (VEC ? 4 : 1)) + (VEC ? e : 0));
+    }
 };
+
+// A wave's rows of an activation: RPW rows of every tile
+template <typename T, bool VEC>
+struct Rows {
+    const char* base;  // the wave's first row of the current tile
+    unsigned step;     // bytes from row to row, less than 2^24
+    __device__ __forceinline__ Rows(const void* p, long bs, long ts, int b, int row)
+        : base((const char*)p + (b * bs + row * ts) * (long)sizeof(T)), step((unsigned)(ts * (long)sizeof(T))) {}
+    __device__ __forceinline__ void move(int tiles) { base += (long)(tiles * TS) * (long)step; }
+    // `row0`: the wave's first row; rows behind the last one, T - 1, read that one: no branch between the loads
+    __device__ __forceinline__ void load(Quad<T>& o, const Elems<VEC>& el, unsigned d0, int row0, int T_) const {
+        const int over = max(0, row0 - (T_ - 1)), most = T_ - 1 - (row0 - over);
+        const char* b = base - (long)(over * (int)step);
+        if (VEC) {
+            const unsigned off = __umul24((unsigned)min(el.lane >> 4, most), step) + d0 * (unsigned)sizeof(T);
+            o = *(const Quad<T>*)(sq_scalar(b) + off);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = at<T>(b + (long)(min(e, most) * (int)step), d0);
+        }
+    }
+};
+// the outputs' rows, packed: `base` the wave's first row of the tile
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_elems(char* base, unsigned step, const Elems<VEC>& el, unsigned d0, int row0, int T_, const float (&v)[4]) {
+    if (VEC) {
+        if (el.ok() && row0 + (el.lane >> 4) < T_) {
+            Quad<T> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = (T)v[e];
+            *(Quad<T>*)(sq_scalar(base) + (__umul24((unsigned)el.lane >> 4, step) + d0 * (unsigned)sizeof(T))) = o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (el.ok() && row0 + e < T_) at<T>((void*)(base + (long)(e * (int)step)), d0) = (T)v[e];
+    }
+}
+// values of the four elements to / from a [TS][64] array in LDS
+template <bool VEC>
+__device__ __forceinline__ void put(float (*a)[64], const Elems<VEC>& el, const float (&v)[4]) {
+    if (VEC) *(float4*)&a[el.row(0)][el.ch(0)] = make_float4(v[0], v[1], v[2], v[3]);
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[el.row(e)][el.ch(e)] = v[e];
+}
+template <bool VEC>
+__device__ __forceinline__ void put2(float2 (*a)[64], const Elems<VEC>& el, const float (&x)[4], const float (&y)[4]) {
+    if (VEC) {
+        float4* p = (float4*)&a[el.row(0)][el.ch(0)];
+        p[0] = make_float4(x[0], y[0], x[1], y[1]);
+        p[1] = make_float4(x[2], y[2], x[3], y[3]);
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[el.row(e)][el.ch(e)] = make_float2(x[e], y[e]);
+}
+// the four waves' values added up
+template <bool VEC>
+__device__ __forceinline__ void get_sum(float (&o)[4], float (*a)[TS][64], const Elems<VEC>& el) {
+    if (VEC) {
+        const int r = el.row(0), c = el.ch(0);
+        const float4 p = *(const float4*)&a[0][r][c], q = *(const float4*)&a[1][r][c], s = *(const float4*)&a[2][r][c], t = *(const float4*)&a[3][r][c];
+        o[0] = (p.x + q.x) + (s.x + t.x), o[1] = (p.y + q.y) + (s.y + t.y), o[2] = (p.z + q.z) + (s.z + t.z), o[3] = (p.w + q.w) + (s.w + t.w);
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = el.row(e), c = el.ch(e);
+            o[e] = (a[0][r][c] + a[1][r][c]) + (a[2][r][c] + a[3][r][c]);
+        }
+}
+template <bool VEC>
+__device__ __forceinline__ void get_sum2(float (&x)[4], float (&y)[4], float2 (*a)[TS][64], const Elems<VEC>& el) {
+    if (VEC) {
+        const int r = el.row(0), c = el.ch(0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = *(const float4*)&a[k][r][c + 2 * h];
+            x[2 * h] = (v[0].x + v[1].x) + (v[2].x + v[3].x), y[2 * h] = (v[0].y + v[1].y) + (v[2].y + v[3].y);
+            x[2 * h + 1] = (v[0].z + v[1].z) + (v[2].z + v[3].z), y[2 * h + 1] = (v[0].w + v[1].w) + (v[2].w + v[3].w);
+        }
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = el.row(e), c = el.ch(e);
+            const float2 p = a[0][r][c], q = a[1][r][c], s = a[2][r][c], t = a[3][r][c];
+            x[e] = (p.x + q.x) + (s.x + t.x), y[e] = (p.y + q.y) + (s.y + t.y);
+        }
+}
 
 // carry[s] <- exp(A sum of steps) carry[s] + end of state n0 + s, over the chunks from, from + dir, ... (count of them), several loads in flight
 template <int K>
@@ -141,18 +240,26 @@ __device__ __forceinline__ void chain(float (&carry)[K], const float (&A2)[K], c
 
 // ENDS: only the state that each chunk but the last leaves behind when it starts from zero, and the sum of its steps
 // (the chunk's decay is exp(A * that sum)).  Otherwise the outputs, each chunk from the states of the chunks before it.
-template <typename T, int NS, bool ENDS, bool HASZ>
+template <typename T, int NS, bool ENDS, bool HASZ, bool VEC>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     const ga_scan_params& p = a.p;
     const Plan& q = a.q;
     // rows whose B and C are in scalar registers at a time, twice (one set on its way)
     constexpr int U = ENDS ? (NS <= 4 ? 4 : NS <= 8 ? 2 : 1) : (NS <= 4 ? 2 : 1);
-    __shared__ float2 sd[TS][64];
-    __shared__ float sy[ENDS ? 1 : 4][ENDS ? 1 : TS][64];
+    __shared__ __attribute__((aligned(16))) float2 sd[TS][64];
+    __shared__ __attribute__((aligned(16))) float sy[ENDS ? 1 : 4][ENDS ? 1 : TS][64];
     const Place x = place(q, ENDS ? q.chunks - 1 : q.chunks, 0, p.G, p.T, p.lengths);
     const int lane = x.lane, w = x.w, len = x.len;
     const unsigned d = x.d;
-    const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
+    const Elems<VEC> el(x, q);
+    const unsigned d0 = el.d(0);
+    float bias[4], Dd[4], total[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias[e] = p.delta_bias ? p.delta_bias[el.d(e)] : 0.f;
+        Dd[e] = !ENDS && p.D ? p.D[el.d(e)] : 0.f;
+        total[e] = 0.f;
+    }
     float A2[NS], h[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -162,20 +269,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
         if (!ENDS && p.state && n < p.N) h[s] = p.state[((size_t)x.b * p.C + d) * p.N + n];
     }
     const int row0 = x.tile0 * TS + w * RPW;
-    Rows us(p.u, sizeof(T), p.u_bs, p.u_ts, x.b, row0), ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0),
-        zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0);
-    char* yp = (char*)p.y + (((size_t)x.b * p.T + row0) * p.C) * sizeof(T);
-    const int ystep = p.C * (int)sizeof(T);
-    T ru[RPW], rd[RPW], rz[RPW];
-    float total = 0.f;
+    Rows<T, VEC> us(p.u, p.u_bs, p.u_ts, x.b, row0), ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0);
+    const unsigned ystep = (unsigned)p.C * (unsigned)sizeof(T);
+    char* yp = (char*)p.y + ((size_t)x.b * p.T + row0) * ystep;
+    Quad<T> ru, rd, rz;
     auto load = [&](int tile) __attribute__((always_inline)) {
-        const int most = p.T - 1 - (tile * TS + w * RPW);
-#pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            ru[r] = at<T>(us.row(r, most), d);
-            rd[r] = at<T>(ds.row(r, most), d);
-            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
-        }
+        us.load(ru, el, d0, tile * TS + w * RPW, p.T);
+        ds.load(rd, el, d0, tile * TS + w * RPW, p.T);
+        if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
     };
     load(x.tile0);
     if (!ENDS) chain<NS>(h, A2, p.ends, p.ends_step, q, p.C, x.b, w * NS, d, 0, 1, x.chunk);
@@ -189,18 +290,19 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
             for (int j = 0; j < (ENDS ? NS : 2 * NS); ++j) o[i][j] = from[i * 2 * NS + j];
     };
     for (int tile = x.tile0; tile < x.tile1; ++tile) {
-        float cu[RPW], cz[RPW];
+        float cu[4], cz[4], step[4], su[4];
+        bool live[4];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = x.ok && t < len;
-            const float raw = (float)rd[r] + bias;
-            const float soft = sq_softplus(raw), step = live ? p.softplus ? soft : raw : 0.f;
-            cu[r] = live ? (float)ru[r] : 0.f;
-            cz[r] = HASZ ? (float)rz[r] : 0.f;
-            total += step;
-            sd[row][lane] = make_float2(step, step * cu[r]);
+        for (int e = 0; e < 4; ++e) {
+            live[e] = el.ok() && tile * TS + el.row(e) < len;
+            const float raw = (float)rd.v[e] + bias[e], soft = sq_softplus(raw);
+            step[e] = live[e] ? p.softplus ? soft : raw : 0.f;
+            cu[e] = live[e] ? (float)ru.v[e] : 0.f;
+            cz[e] = HASZ ? (float)rz.v[e] : 0.f;
+            total[e] += step[e];
+            su[e] = step[e] * cu[e];
         }
+        put2(sd, el, step, su);
         fetch(m[0], mp);
         __syncthreads();
         if (tile + 1 < x.tile1) {
@@ -244,15 +346,17 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
             for (int t = 0; t < TS; ++t) sy[w][t][lane] = y[t];
         }
         __syncthreads();
-        if (!ENDS) {
+        if constexpr (!ENDS) {
+            float o[4];
+            get_sum(o, sy, el);
 #pragma unroll
-            for (int r = 0; r < RPW; ++r) {
-                const int row = w * RPW + r, t = tile * TS + row;
-                float o = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                if (HASZ) o *= sq_silu(cz[r]);
-                if (x.ok && t < p.T) at<T>((void*)(yp + (long)(r * ystep)), d) = (T)(t < len ? o : 0.f);
+            for (int e = 0; e < 4; ++e) {
+                o[e] = fmaf(Dd[e], cu[e], o[e]);
+                if (HASZ) o[e] *= sq_silu(cz[e]);
+                o[e] = live[e] ? o[e] : 0.f;
             }
-            yp += (long)TS * ystep;
+            store_elems<T>(yp, ystep, el, d0, tile * TS + w * RPW, p.T, o);
+            yp += (size_t)TS * ystep;
         }
     }
     if (ENDS) {
@@ -261,9 +365,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + w * NS + s) * p.C + d] = h[s];
         }
-        sd[w][lane].x = total;
+        put2(sd, el, total, total);
         __syncthreads();
-        if (w == 0 && x.ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
+        if (w == 0 && x.ok) {
+            float v = 0.f;
+#pragma unroll
+            for (int t = 0; t < TS; ++t) v += sd[t][lane].x;
+            p.ends_step[e * p.C + d] = v;
+        }
     } else if (p.last && x.chunk == q.chunks - 1 && x.ok) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -275,16 +384,23 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
 
 // The adjoint that each chunk but the first hands to the one before it when nothing comes in from behind:
 //   g_t = carry + C_t dyg_t, carry = exp(D_t A) g_t, from the chunk's last row to its first
-template <typename T, int NS, bool HASZ>
+template <typename T, int NS, bool HASZ, bool VEC>
 __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int U = NS <= 4 ? 4 : NS <= 8 ? 2 : 1;
-    __shared__ float2 sd[TS][64];
+    __shared__ __attribute__((aligned(16))) float2 sd[TS][64];
     const Place x = place(q, q.chunks - 1, 1, p.G, p.T, p.lengths);
     const int lane = x.lane, w = x.w, len = x.len;
     const unsigned d = x.d;
-    const float bias = p.delta_bias ? p.delta_bias[d] : 0.f;
+    const Elems<VEC> el(x, q);
+    const unsigned d0 = el.d(0);
+    float bias[4], total[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias[e] = p.delta_bias ? p.delta_bias[el.d(e)] : 0.f;
+        total[e] = 0.f;
+    }
     float A2[NS], c[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -293,18 +409,12 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
         c[s] = 0.f;
     }
     const int row0 = (x.tile1 - 1) * TS + w * RPW;
-    Rows ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0),
-        gs(p.dy, sizeof(T), (long)p.T * p.C, p.C, x.b, row0);
-    T rd[RPW], rz[RPW], rg[RPW];
-    float total = 0.f;
+    Rows<T, VEC> ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0), gs(p.dy, (long)p.T * p.C, p.C, x.b, row0);
+    Quad<T> rd, rz, rg;
     auto load = [&](int tile) __attribute__((always_inline)) {
-        const int most = p.T - 1 - (tile * TS + w * RPW);
-#pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            rd[r] = at<T>(ds.row(r, most), d);
-            rg[r] = at<T>(gs.row(r, most), d);
-            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
-        }
+        ds.load(rd, el, d0, tile * TS + w * RPW, p.T);
+        gs.load(rg, el, d0, tile * TS + w * RPW, p.T);
+        if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
     };
     load(x.tile1 - 1);
     float m[2][U][NS];
@@ -317,17 +427,18 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     };
     for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
+        float step[4], dy[4];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = x.ok && t < len;
-            const float raw = (float)rd[r] + bias;
-            const float soft = sq_softplus(raw), step = live ? p.softplus ? soft : raw : 0.f;
-            float dy = (float)rg[r];
-            if (HASZ) dy *= sq_silu((float)rz[r]);
-            total += step;
-            sd[row][lane] = make_float2(step, live ? dy : 0.f);
+        for (int e = 0; e < 4; ++e) {
+            const bool live = el.ok() && tile * TS + el.row(e) < len;
+            const float raw = (float)rd.v[e] + bias[e], soft = sq_softplus(raw);
+            step[e] = live ? p.softplus ? soft : raw : 0.f;
+            dy[e] = (float)rg.v[e];
+            if (HASZ) dy[e] *= sq_silu((float)rz.v[e]);
+            dy[e] = live ? dy[e] : 0.f;
+            total[e] += step[e];
         }
+        put2(sd, el, step, dy);
         fetch(m[0], mp + (TS - U) * 2 * NS);
         __syncthreads();
         if (tile > x.tile0) {
@@ -360,35 +471,53 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) p.ends[(e * q.NP + w * NS + s) * p.C + d] = c[s];
     }
-    sd[w][lane].x = total;
+    put2(sd, el, total, total);
     __syncthreads();
-    if (w == 0 && x.ok) p.ends_step[e * p.C + d] = (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x);
+    if (w == 0 && x.ok) {
+        float v = 0.f;
+#pragma unroll
+        for (int t = 0; t < TS; ++t) v += sd[t][lane].x;
+        p.ends_step[e * p.C + d] = v;
+    }
 }
 
 // Per tile, from the last to the first: the states again from the one saved at the tile's start (kept in registers, with the decays), then
 // the adjoint backwards through them; NB states of a wave at a time.  With more than NB the adjoint, dA and the rows' values wait in LDS for their turn: a
 // vector register spilled here is not only slow (the compiler has been seen to place such copies under a branch's mask).
-template <typename T, int NS, bool HASZ>
+template <typename T, int NS, bool HASZ, bool VEC>
 __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs a) {
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int NB = NS < 4 ? NS : 4, SB = NS / NB, U = 2;
-    __shared__ float2 sd[TS][64];     // step, step * u
-    __shared__ float sg[TS][64];      // dy * gate
-    __shared__ float sy[4][TS][64];   // <C, h> over a wave's states
-    __shared__ float2 ss[4][TS][64];  // <g, B>, <g a h_prev, A>
+    constexpr bool AHEAD = SB == 1 && VEC;  // registers for the next tile's rows on their way
+    __shared__ __attribute__((aligned(16))) float2 sd[TS][64];     // step, step * u
+    __shared__ __attribute__((aligned(16))) float sg[TS][64];      // dy * gate
+    __shared__ __attribute__((aligned(16))) float sy[4][TS][64];   // <C, h> over a wave's states
+    __shared__ __attribute__((aligned(16))) float2 ss[4][TS][64];  // <g, B>, <g a h_prev, A>
     __shared__ float sm[4][TS][2 * NS];
-    __shared__ float wait[SB > 1 ? 2 * NS + 7 * RPW : 1][SB > 1 ? 256 : 1];
+    __shared__ float wait[SB > 1 ? 2 * NS + 28 : 1][SB > 1 ? 256 : 1];
     const Place x = place(q, q.chunks, 0, p.G, p.T, p.lengths);
     const int lane = x.lane, w = x.w, len = x.len;
     const unsigned d = x.d;
-    const float bias = p.delta_bias ? p.delta_bias[d] : 0.f, Dd = p.D ? p.D[d] : 0.f;
+    const Elems<VEC> el(x, q);
+    const unsigned d0 = el.d(0);
+    float bias[4], Dd[4], dD[4], dbias[4];
+    auto load_params = [&](const float* pb, const float* pD) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (pb) bias[e] = pb[el.d(e)];
+            if (pD) Dd[e] = pD[el.d(e)];
+        }
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = Dd[e] = dD[e] = dbias[e] = 0.f;
+    if (SB == 1) load_params(p.delta_bias, p.D);
     const int row0 = (x.tile1 - 1) * TS + w * RPW;
-    Rows us(p.u, sizeof(T), p.u_bs, p.u_ts, x.b, row0), ds(p.delta, sizeof(T), p.delta_bs, p.delta_ts, x.b, row0),
-        zs(p.z, sizeof(T), p.z_bs, p.z_ts, x.b, row0), gs(p.dy, sizeof(T), (long)p.T * p.C, p.C, x.b, row0);
-    size_t orow = ((size_t)x.b * p.T + row0) * p.C * sizeof(T);  // of the outputs, in bytes
-    const int ostep = p.C * (int)sizeof(T);
-    T ru[RPW], rd[RPW], rz[RPW], rg[RPW];
+    Rows<T, VEC> us(p.u, p.u_bs, p.u_ts, x.b, row0), ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0),
+        gs(p.dy, (long)p.T * p.C, p.C, x.b, row0);
+    const unsigned ostep = (unsigned)p.C * (unsigned)sizeof(T);
+    size_t orow = ((size_t)x.b * p.T + row0) * ostep;  // of the outputs, in bytes
+    Quad<T> ru, rd, rz, rg;
     float hn[NB];
     auto load_h = [&](int tile, int sb) __attribute__((always_inline)) {
         const float* hp = p.hs + (((size_t)x.b * q.tiles + tile) * q.NP + w * NS + sb * NB) * p.C;
@@ -397,16 +526,13 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
     };
     auto load = [&](int tile) __attribute__((always_inline)) {
         load_h(tile, 0);
-        const int most = p.T - 1 - (tile * TS + w * RPW);
-#pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            ru[r] = at<T>(us.row(r, most), d);
-            rd[r] = at<T>(ds.row(r, most), d);
-            rg[r] = at<T>(gs.row(r, most), d);
-            if (HASZ) rz[r] = at<T>(zs.row(r, most), d);
-        }
+        const int first = tile * TS + w * RPW;
+        us.load(ru, el, d0, first, p.T);
+        ds.load(rd, el, d0, first, p.T);
+        gs.load(rg, el, d0, first, p.T);
+        if (HASZ) zs.load(rz, el, d0, first, p.T);
     };
-    if (SB == 1) load(x.tile1 - 1);
+    if (AHEAD) load(x.tile1 - 1);
     float A2[NB], c[NB], dA[NB];
     auto load_A = [&](int sb) __attribute__((always_inline)) {
 #pragma unroll
@@ -434,44 +560,48 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
             }
         }
     }
-    float dD = 0.f, dbias = 0.f;
     // what only a tile's end needs is read again from the kernel's arguments there: kept over the loop it costs the scalar registers of B and C
     const __attribute__((address_space(4))) BwdArgs* args = (const __attribute__((address_space(4))) BwdArgs*)__builtin_amdgcn_kernarg_segment_ptr();
     for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
-        float cu[RPW], cslope[RPW], cz[RPW], csig[RPW], cdy[RPW], cstep[RPW], cg[RPW], h0[NB];
-        if (SB > 1) load(tile);
+        float cu[4], cslope[4], cz[4], csig[4], cdy[4], cstep[4], cg[4], su[4], h0[NB];
+        if (!AHEAD) load(tile);
+        if (SB > 1) {
+            const float* pb = p.delta_bias;
+            asm volatile("" : "+s"(pb));  // (loaded here and not kept over the loop)
+            load_params(pb, nullptr);
+        }
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = x.ok && t < len;
-            const float raw = (float)rd[r] + bias;
+        for (int e = 0; e < 4; ++e) {
+            const bool live = el.ok() && tile * TS + el.row(e) < len;
+            const float raw = (float)rd.v[e] + bias[e];
             float slope;
             const float soft = sq_softplus(raw, slope), step = p.softplus ? soft : raw;
-            cslope[r] = p.softplus ? slope : 1.f;
-            cstep[r] = live ? step : 0.f;
-            cu[r] = live ? (float)ru[r] : 0.f;
-            cdy[r] = live ? (float)rg[r] : 0.f;
-            cz[r] = HASZ && live ? (float)rz[r] : 0.f;
-            csig[r] = HASZ ? sq_sigmoid(cz[r]) : 1.f;
-            cg[r] = HASZ ? cdy[r] * (cz[r] * csig[r]) : cdy[r];
-            sd[row][lane] = make_float2(cstep[r], cstep[r] * cu[r]);
-            sg[row][lane] = cg[r];
+            cslope[e] = live ? p.softplus ? slope : 1.f : 0.f;
+            cstep[e] = live ? step : 0.f;
+            cu[e] = live ? (float)ru.v[e] : 0.f;
+            cdy[e] = live ? (float)rg.v[e] : 0.f;
+            cz[e] = HASZ && live ? (float)rz.v[e] : 0.f;
+            csig[e] = HASZ ? sq_sigmoid(cz[e]) : 1.f;
+            cg[e] = HASZ ? cdy[e] * (cz[e] * csig[e]) : cdy[e];
+            su[e] = cstep[e] * cu[e];
         }
+        put2(sd, el, cstep, su);
+        put(sg, el, cg);
         if (SB == 1) {
 #pragma unroll
             for (int j = 0; j < NB; ++j) h0[j] = hn[j];
         } else {
 #pragma unroll
-            for (int r = 0; r < RPW; ++r) {
-                float* keep = &wait[2 * NS + 7 * r][threadIdx.x];
-                keep[0] = cu[r], keep[256] = cslope[r], keep[512] = cz[r], keep[768] = csig[r], keep[1024] = cdy[r], keep[1280] = cstep[r], keep[1536] = cg[r];
+            for (int e = 0; e < 4; ++e) {
+                float* keep = &wait[2 * NS + 7 * e][threadIdx.x];
+                keep[0] = cu[e], keep[256] = cslope[e], keep[512] = cz[e], keep[768] = csig[e], keep[1024] = cdy[e], keep[1280] = cstep[e], keep[1536] = cg[e];
             }
         }
         __syncthreads();
         if (tile > x.tile0) {
             us.move(-1), ds.move(-1), zs.move(-1), gs.move(-1);
-            if (SB == 1) load(tile - 1);  // (with more states there is no room for rows on their way)
+            if (AHEAD) load(tile - 1);
         }
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) {
@@ -500,10 +630,17 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                     v[set][i] = sd[t0 + i][lane];
                 }
             };
+            float gy[2][U];
+            auto fetch_back = [&](int set, int t0) __attribute__((always_inline)) {
+                fetch(set, t0);
+#pragma unroll
+                for (int i = 0; i < U; ++i) gy[set][i] = sg[t0 + i][lane];
+            };
             fetch(0, 0);
 #pragma unroll
             for (int k = 0; k < TS / U; ++k) {
                 if (k + 1 < TS / U) fetch((k + 1) & 1, (k + 1) * U);
+                else fetch_back(0, TS - U);  // the way back starts where this one ends
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < U; ++i) {
@@ -521,13 +658,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            float gy[2][U];
-            auto fetch_back = [&](int set, int t0) __attribute__((always_inline)) {
-                fetch(set, t0);
-#pragma unroll
-                for (int i = 0; i < U; ++i) gy[set][i] = sg[t0 + i][lane];
-            };
-            fetch_back(0, TS - U);
+            static_assert(TS / U % 2 == 0, "the first set is free at the end");
             // a row's 2 NB products are folded until a lane has one, summed over 2 NB lanes; KEEP rows of these then over the other lanes
             constexpr int KEEP = TS < 64 / (2 * NB) ? TS : 64 / (2 * NB);
             float part[KEEP];
@@ -580,33 +711,28 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
         const auto& pc = args->p;
         if (SB > 1) {
 #pragma unroll
-            for (int r = 0; r < RPW; ++r) {
-                const float* keep = &wait[2 * NS + 7 * r][threadIdx.x];
-                cu[r] = keep[0], cslope[r] = keep[256], cz[r] = keep[512], csig[r] = keep[768], cdy[r] = keep[1024], cstep[r] = keep[1280], cg[r] = keep[1536];
+            for (int e = 0; e < 4; ++e) {
+                const float* keep = &wait[2 * NS + 7 * e][threadIdx.x];
+                cu[e] = keep[0], cslope[e] = keep[256], cz[e] = keep[512], csig[e] = keep[768], cdy[e] = keep[1024], cstep[e] = keep[1280], cg[e] = keep[1536];
             }
         }
+        if (SB > 1) load_params(nullptr, pc.D);
+        float s1[4], s2[4], y[4], du[4], dd[4], dz[4];
+        get_sum2(s1, s2, ss, el);
+        if (HASZ) get_sum(y, sy, el);
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            const int row = w * RPW + r, t = tile * TS + row;
-            const bool live = x.ok && t < len;
-            const float2 x0 = ss[0][row][lane], x1 = ss[1][row][lane], x2 = ss[2][row][lane], x3 = ss[3][row][lane];
-            const float s1 = (x0.x + x1.x) + (x2.x + x3.x), s2 = ((x0.y + x1.y) + (x2.y + x3.y)) * SQ_LN2;
-            const float du = fmaf(cstep[r], s1, Dd * cg[r]), dd = live ? fmaf(cu[r], s1, s2) * cslope[r] : 0.f;
-            dD = fmaf(cg[r], cu[r], dD);
-            dbias += dd;
-            float dz = 0.f;
-            if (HASZ) {
-                const float y = fmaf(Dd, cu[r], (sy[0][row][lane] + sy[1][row][lane]) + (sy[2][row][lane] + sy[3][row][lane]));
-                dz = cdy[r] * y * csig[r] * fmaf(cz[r], 1.f - csig[r], 1.f);
-            }
-            if (t < p.T && x.ok) {
-                const size_t o = orow + (long)(r * ostep);
-                at<T>((void*)((char*)pc.du + o), d) = (T)(live ? du : 0.f);
-                at<T>((void*)((char*)pc.ddelta + o), d) = (T)dd;
-                if (HASZ) at<T>((void*)((char*)pc.dz + o), d) = (T)(live ? dz : 0.f);
-            }
+        for (int e = 0; e < 4; ++e) {  // (behind an item's end cstep, cg, cslope, cdy are zero, and with them what is stored)
+            du[e] = fmaf(cstep[e], s1[e], Dd[e] * cg[e]);
+            dd[e] = fmaf(cu[e], s1[e], s2[e] * SQ_LN2) * cslope[e];
+            dD[e] = fmaf(cg[e], cu[e], dD[e]);
+            dbias[e] += dd[e];
+            dz[e] = HASZ ? cdy[e] * fmaf(Dd[e], cu[e], y[e]) * csig[e] * fmaf(cz[e], 1.f - csig[e], 1.f) : 0.f;
         }
-        orow -= (long)TS * ostep;
+        const int first = tile * TS + w * RPW;
+        store_elems<T>((char*)pc.du + orow, ostep, el, d0, first, p.T, du);
+        store_elems<T>((char*)pc.ddelta + orow, ostep, el, d0, first, p.T, dd);
+        if (HASZ) store_elems<T>((char*)pc.dz + orow, ostep, el, d0, first, p.T, dz);
+        orow -= (size_t)TS * ostep;
         // this block's share of dB and dC, in the layout of the maps
         const int slab = (blockIdx.x % q.nCb) % q.cbg;
         float* mo = pc.dmaps + ((size_t)slab * pc.B * pc.G * q.tiles + x.item + tile) * (4 * TS * 2 * NS);
@@ -615,7 +741,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
             const int k = i * 256 + threadIdx.x;
             if (4 * TS * 2 * NS % 256 == 0 || k < 4 * TS * 2 * NS) at<float>(mo, (unsigned)k) = (&sm[0][0][0])[k];
         }
-        __syncthreads();
+        // (no barrier: what the next tile writes before its first one is read here by nobody but its writer, or before the one above)
     }
     const size_t e = (size_t)x.b * q.chunks + x.chunk;
 #pragma unroll
@@ -630,11 +756,13 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
             }
         }
     }
-    sd[w][lane] = make_float2(dD, dbias);
+    __syncthreads();
+    put2(sd, el, dD, dbias);
     __syncthreads();
     if (w < 2 && x.ok) {
-        const float v = w == 0 ? (sd[0][lane].x + sd[1][lane].x) + (sd[2][lane].x + sd[3][lane].x)
-                               : (sd[0][lane].y + sd[1][lane].y) + (sd[2][lane].y + sd[3][lane].y);
+        float v = 0.f;
+#pragma unroll
+        for (int t = 0; t < TS; ++t) v += w == 0 ? sd[t][lane].x : sd[t][lane].y;
         p.dparams[(e * (q.NP + 2) + q.NP + w) * p.C + d] = v;
     }
 }
@@ -727,6 +855,8 @@ int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
     return GA_OK;
 }
 
+// whether rows of this tensor (absent: any) can be accessed in quads
+bool quads(const void* p, long bs, long ts, size_t elem) { return !p || (!((uintptr_t)p & (4 * elem - 1)) && bs % 4 == 0 && ts % 4 == 0); }
 bool bad_strides(long a, long b, long c) {
     return a < 0 || b < 0 || c < 0 || a > GA_SCAN_MAX_STRIDE || b > GA_SCAN_MAX_STRIDE || c > GA_SCAN_MAX_STRIDE;
 }
@@ -736,41 +866,46 @@ int grid_for(size_t n) {
     return (int)(g < 4096 ? g : 4096);
 }
 
-template <typename T, int NS>
-int launch_fwd(const Args& a, hipStream_t s) {
+template <typename T, int NS, bool HASZ, bool VEC>
+int launch_fwd_as(const Args& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_fwd_kernel<T, NS, true, false><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_fwd_kernel<T, NS, true, false, VEC><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    if (a.p.z) scan_fwd_kernel<T, NS, false, true><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
-    else scan_fwd_kernel<T, NS, false, false><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    scan_fwd_kernel<T, NS, false, HASZ, VEC><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
+template <typename T, int NS>
+int launch_fwd(const Args& a, hipStream_t s) {
+    if (a.vec) return a.p.z ? launch_fwd_as<T, NS, true, true>(a, s) : launch_fwd_as<T, NS, false, true>(a, s);
+    return a.p.z ? launch_fwd_as<T, NS, true, false>(a, s) : launch_fwd_as<T, NS, false, false>(a, s);
+}
 
-template <typename T, int NS, bool HASZ>
-int launch_bwd_z(const BwdArgs& a, hipStream_t s) {
+template <typename T, int NS, bool HASZ, bool VEC>
+int launch_bwd_as(const BwdArgs& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
-        scan_bwd_ends_kernel<T, NS, HASZ><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
+        scan_bwd_ends_kernel<T, NS, HASZ, VEC><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
     }
-    scan_bwd_kernel<T, NS, HASZ><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
+    scan_bwd_kernel<T, NS, HASZ, VEC><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
 template <typename T, int NS>
 int launch_bwd(const BwdArgs& a, hipStream_t s) {
-    return a.p.z ? launch_bwd_z<T, NS, true>(a, s) : launch_bwd_z<T, NS, false>(a, s);
+    constexpr bool V = NS <= 8;  // (64 states: no registers for quads)
+    if (V && a.vec) return a.p.z ? launch_bwd_as<T, NS, true, V>(a, s) : launch_bwd_as<T, NS, false, V>(a, s);
+    return a.p.z ? launch_bwd_as<T, NS, true, false>(a, s) : launch_bwd_as<T, NS, false, false>(a, s);
 }
 
 #define SCAN_DISPATCH(FN, T, ARGS)                 \
     (ARGS.q.NS == 16  ? FN<T, 16>(ARGS, s)         \
      : ARGS.q.NS == 8 ? FN<T, 8>(ARGS, s)          \
      : ARGS.q.NS == 4 ? FN<T, 4>(ARGS, s)          \
-     : ARGS.q.NS == 2 ? FN<T, 2>(ARGS, s)          \
-                      : FN<T, 1>(ARGS, s))
+                      : FN<T, 2>(ARGS, s))
 
 template <typename T>
 int fwd(const Args& a, hipStream_t s) {
@@ -815,10 +950,13 @@ int ga_scan_fwd(const ga_scan_params* hp, int dtype, hipStream_t s) {
     const ga_scan_params& p = *hp;
     const int rc = bad_sizes(p.B, p.T, p.C, p.N, p.G, dtype);
     if (rc) return rc;
-    const Args a{p, make_plan(p.B, p.T, p.C, p.N, p.G)};
+    Args a{p, make_plan(p.B, p.T, p.C, p.N, p.G), 0};
     if (!p.u || !p.delta || !p.A || !p.Bm || !p.Cm || !p.y || !p.maps || (a.q.chunks > 1 && (!p.ends || !p.ends_step))) return GA_ERR_ARG;
     if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
+    const size_t el = dtype == GA_DTYPE_BF16 ? 2 : 4;
+    a.vec = a.q.Cg % 4 == 0 && quads(p.u, p.u_bs, p.u_ts, el) && quads(p.delta, p.delta_bs, p.delta_ts, el) && quads(p.z, p.z_bs, p.z_ts, el) &&
+            quads(p.y, 0, 0, el);
     return dtype == GA_DTYPE_BF16 ? fwd<bf16_t>(a, s) : fwd<float>(a, s);
 }
 
@@ -827,12 +965,15 @@ int ga_scan_bwd(const ga_scan_bwd_params* hp, int dtype, hipStream_t s) {
     const ga_scan_bwd_params& p = *hp;
     const int rc = bad_sizes(p.B, p.T, p.C, p.N, p.G, dtype);
     if (rc) return rc;
-    const BwdArgs a{p, make_plan(p.B, p.T, p.C, p.N, p.G)};
+    BwdArgs a{p, make_plan(p.B, p.T, p.C, p.N, p.G), 0};
     if (!p.u || !p.delta || !p.A || !p.dy || !p.maps || !p.hs || !p.du || !p.ddelta || !p.dA || !p.dBm || !p.dCm || !p.dmaps || !p.dparams ||
         (!p.z) != (!p.dz) || (a.q.chunks > 1 && (!p.ends || !p.ends_step)))
         return GA_ERR_ARG;
     if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
+    const size_t el = dtype == GA_DTYPE_BF16 ? 2 : 4;
+    a.vec = a.q.Cg % 4 == 0 && quads(p.u, p.u_bs, p.u_ts, el) && quads(p.delta, p.delta_bs, p.delta_ts, el) && quads(p.z, p.z_bs, p.z_ts, el) &&
+            quads(p.dy, 0, 0, el) && quads(p.du, 0, 0, el) && quads(p.ddelta, 0, 0, el) && quads(p.dz, 0, 0, el);
     return dtype == GA_DTYPE_BF16 ? bwd<bf16_t>(a, s) : bwd<float>(a, s);
 }
 

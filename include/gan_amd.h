@@ -560,7 +560,7 @@ int ga_causal_conv_step(const ga_causal_conv_step_params* h_params, int dtype, g
  * fp32 (the last two may be NULL); state [B][C][N] fp32 (NULL: zero); last [B][C][N] (may be NULL) receives the state at the item's end.
  * maps / hs / ends / ends_step: fp32 buffers of ga_scan_sizes() elements; maps and hs are what the backward pass reads (hs NULL: not wanted). */
 #define GA_SCAN_MAX_STATES 64
-#define GA_SCAN_MAX_STRIDE (1 << 24) /* elements from a row to the next, and channels, at the most */
+#define GA_SCAN_MAX_STRIDE ((1 << 22) - 1) /* elements from a row to the next, and channels, at the most */
 typedef struct ga_scan_buffers {
     size_t maps;      /* B and C in float32, in the kernels' order */
     size_t hs;        /* the state at every 16th row */
