@@ -11,7 +11,7 @@ namespace {
 
 constexpr int TS = 16;          // rows of a tile
 constexpr int RPW = TS / 4;     // rows that one wave prepares and finishes
-constexpr int MAX_CHUNKS = 64;  // a block adds up the chunks before (behind) its own one by one
+constexpr int MAX_CHUNKS = 256;
 
 typedef const __attribute__((address_space(4))) float* uniform_ptr;
 // `p` as a value that the compiler cannot trace: loads through it are issued where they stand, and not all at once at the top (their results
@@ -37,7 +37,10 @@ Plan make_plan(int B, int T, int C, int N, int G) {
     q.nCb = q.cbg * G;
     q.tiles = (T + TS - 1) / TS;
     const long blocks = (long)B * q.nCb;
-    long want = (1024 + blocks - 1) / blocks;  // four blocks a CU
+    // Chunks for four blocks a CU, and for eight where a chunk is still long enough (16 tiles) not to notice its start: at 16 x 2250 x 1024 the
+    // forward kernel takes 247 us with two blocks a CU, 201 with four, 181 with eight; a 2250-row prompt of 8 blocks 37 us with four, 51 with eight.
+    long want = (1024 + blocks - 1) / blocks;
+    if (q.tiles / want >= 16) want = (2048 + blocks - 1) / blocks;
     if (want > MAX_CHUNKS) want = MAX_CHUNKS;
     if (want > q.tiles) want = q.tiles;
     if (want < 1) want = 1;
@@ -81,6 +84,7 @@ __global__ __launch_bounds__(256) void scan_maps_kernel(const T* __restrict__ Bm
 // Where a block and a lane are.  `d` counts channels, unsigned so that an address is a scalar base plus a 32-bit offset.
 struct Place {
     int lane, w, chunk, b, g, len, tile0, tile1;
+    int end;  // tile1, or the tile behind the item's last row where that comes first: nothing happens in the tiles from there on
     unsigned d;
     bool ok;
     size_t item;  // first tile of the item's group in the maps
@@ -99,6 +103,7 @@ __device__ __forceinline__ Place place(const Plan& q, int nch, int first_chunk, 
     x.len = sq_len(lengths, x.b, T);
     x.tile0 = x.chunk * q.chunk_tiles;
     x.tile1 = min(x.tile0 + q.chunk_tiles, q.tiles);
+    x.end = max(x.tile0, min(x.tile1, (x.len + TS - 1) / TS));
     x.item = (size_t)(x.b * G + x.g) * q.tiles;
     return x;
 }
@@ -215,25 +220,34 @@ __device__ __forceinline__ void get_sum2(float (&x)[4], float (&y)[4], float2 (*
         }
 }
 
-// carry[s] <- exp(A sum of steps) carry[s] + end of state n0 + s, over the chunks from, from + dir, ... (count of them), several loads in flight
-template <int K>
-__device__ __forceinline__ void chain(float (&carry)[K], const float (&A2)[K], const float* ends, const float* ends_step, const Plan& q, int C, int b,
-                                      int n0, unsigned d, int from, int dir, int count) {
-    constexpr int U = K <= 4 ? 8 : K <= 8 ? 4 : 2;
-    for (int k = 0; k < count; k += U) {
-        float sum[U], end[U][K];
+// What comes into each chunk, from what each one leaves behind by itself, in place: carry' = exp(A sum of steps) carry + end, over the chunks
+// in order (forward) or against it (backward: dir < 0), from `first` [B][C][N] (or zero).  A thread is one state of one channel, with the loads
+// of 32 chunks in flight: few threads, a long way to memory.  (As a loop at the start of every block of the main kernel it cost 11 of the 23 us
+// that a prompt of 2250 rows and 8 blocks spent there.)
+__global__ __launch_bounds__(256) void scan_carry_kernel(const float* __restrict__ A, const float* __restrict__ first, float* __restrict__ ends,
+                                                         const float* __restrict__ ends_step, Plan q, int B, int C, int N, int dir) {
+    constexpr int U = 32;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)B * N * C) return;
+    const int d = (int)(i % C), n = (int)(i / C % N), b = (int)(i / C / N);
+    const float A2 = A[(size_t)d * N + n] * SQ_LOG2E;
+    float c = first ? first[((size_t)b * C + d) * N + n] : 0.f;
+    const float* sp = ends_step + (size_t)b * q.chunks * C + d;
+    float* ep = ends + ((size_t)b * q.chunks * q.NP + n) * C + d;
+    for (int k = 0; k < q.chunks; k += U) {
+        float sum[U], end[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const size_t e = (size_t)b * q.chunks + (from + dir * min(k + i, count - 1));
-            sum[i] = at<float>(ends_step + e * C, d);
-#pragma unroll
-            for (int s = 0; s < K; ++s) end[i][s] = at<float>(ends + (e * q.NP + n0 + s) * C, d);
+        for (int u = 0; u < U; ++u) {
+            const int kk = min(k + u, q.chunks - 1), chunk = dir < 0 ? q.chunks - 1 - kk : kk;
+            sum[u] = sp[(size_t)chunk * C];
+            end[u] = ep[(size_t)chunk * q.NP * C];
         }
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (k + i < count) {
-#pragma unroll
-                for (int s = 0; s < K; ++s) carry[s] = fmaf(__builtin_amdgcn_exp2f(sum[i] * A2[s]), carry[s], end[i][s]);
+        for (int u = 0; u < U; ++u)
+            if (k + u < q.chunks) {
+                const int chunk = dir < 0 ? q.chunks - 1 - (k + u) : k + u;
+                ep[(size_t)chunk * q.NP * C] = c;
+                c = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), c, end[u]);  // (of the last chunk: not written by any block, not used)
             }
     }
 }
@@ -264,9 +278,24 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const int n = w * NS + s;
-        A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
+        const float v = p.A[(size_t)d * p.N + min(n, p.N - 1)] * SQ_LOG2E;
+        A2[s] = n < p.N ? v : 0.f;
         h[s] = 0.f;
-        if (!ENDS && p.state && n < p.N) h[s] = p.state[((size_t)x.b * p.C + d) * p.N + n];
+    }
+    if (!ENDS && q.chunks > 1) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int n = w * NS + s;
+            const float v = p.ends[(((size_t)x.b * q.chunks + x.chunk) * q.NP + min(n, p.N - 1)) * p.C + d];
+            h[s] = n < p.N ? v : 0.f;
+        }
+    } else if (!ENDS && p.state) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int n = w * NS + s;
+            const float v = p.state[((size_t)x.b * p.C + d) * p.N + min(n, p.N - 1)];
+            h[s] = n < p.N ? v : 0.f;
+        }
     }
     const int row0 = x.tile0 * TS + w * RPW;
     Rows<T, VEC> us(p.u, p.u_bs, p.u_ts, x.b, row0), ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0);
@@ -279,7 +308,6 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
         if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
     };
     load(x.tile0);
-    if (!ENDS) chain<NS>(h, A2, p.ends, p.ends_step, q, p.C, x.b, w * NS, d, 0, 1, x.chunk);
     uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + x.tile0) * 4 + w) * (TS * 2 * NS));
     float m[2][U][2 * NS];
     auto fetch = [&](float (&o)[U][2 * NS], uniform_ptr at) __attribute__((always_inline)) {
@@ -289,7 +317,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
 #pragma unroll
             for (int j = 0; j < (ENDS ? NS : 2 * NS); ++j) o[i][j] = from[i * 2 * NS + j];
     };
-    for (int tile = x.tile0; tile < x.tile1; ++tile) {
+    for (int tile = x.tile0; tile < x.end; ++tile) {
         float cu[4], cz[4], step[4], su[4];
         bool live[4];
 #pragma unroll
@@ -305,7 +333,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
         put2(sd, el, step, su);
         fetch(m[0], mp);
         __syncthreads();
-        if (tile + 1 < x.tile1) {
+        if (tile + 1 < x.end) {
             us.move(1), ds.move(1), zs.move(1);
             load(tile + 1);
         }
@@ -359,6 +387,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
             yp += (size_t)TS * ystep;
         }
     }
+    if constexpr (!ENDS) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int tile = x.end; tile < x.tile1; ++tile, yp += (size_t)TS * ystep) store_elems<T>(yp, ystep, el, d0, tile * TS + w * RPW, p.T, zero);
+    }
     if (ENDS) {
         const size_t e = (size_t)x.b * q.chunks + x.chunk;
         if (x.ok) {
@@ -405,10 +437,11 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const int n = w * NS + s;
-        A2[s] = n < p.N ? p.A[(size_t)d * p.N + n] * SQ_LOG2E : 0.f;
+        const float v = p.A[(size_t)d * p.N + min(n, p.N - 1)] * SQ_LOG2E;
+        A2[s] = n < p.N ? v : 0.f;
         c[s] = 0.f;
     }
-    const int row0 = (x.tile1 - 1) * TS + w * RPW;
+    const int row0 = max(x.end - 1, 0) * TS + w * RPW;
     Rows<T, VEC> ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0), gs(p.dy, (long)p.T * p.C, p.C, x.b, row0);
     Quad<T> rd, rz, rg;
     auto load = [&](int tile) __attribute__((always_inline)) {
@@ -416,7 +449,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
         gs.load(rg, el, d0, tile * TS + w * RPW, p.T);
         if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
     };
-    load(x.tile1 - 1);
+    load(max(x.end - 1, 0));
     float m[2][U][NS];
     auto fetch = [&](float (&o)[U][NS], uniform_ptr at) __attribute__((always_inline)) {
         uniform_ptr from = here(at);
@@ -425,7 +458,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
 #pragma unroll
             for (int j = 0; j < NS; ++j) o[i][j] = from[i * 2 * NS + NS + j];
     };
-    for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
+    for (int tile = x.end - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
         float step[4], dy[4];
 #pragma unroll
@@ -489,7 +522,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int NB = NS < 4 ? NS : 4, SB = NS / NB, U = 2;
-    constexpr bool AHEAD = SB == 1 && VEC;  // registers for the next tile's rows on their way
+    constexpr bool AHEAD = SB == 1 && VEC && sizeof(T) == 2;  // registers for the next tile's rows on their way
     __shared__ __attribute__((aligned(16))) float2 sd[TS][64];     // step, step * u
     __shared__ __attribute__((aligned(16))) float sg[TS][64];      // dy * gate
     __shared__ __attribute__((aligned(16))) float sy[4][TS][64];   // <C, h> over a wave's states
@@ -512,7 +545,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
 #pragma unroll
     for (int e = 0; e < 4; ++e) bias[e] = Dd[e] = dD[e] = dbias[e] = 0.f;
     if (SB == 1) load_params(p.delta_bias, p.D);
-    const int row0 = (x.tile1 - 1) * TS + w * RPW;
+    const int row0 = max(x.end - 1, 0) * TS + w * RPW;
     Rows<T, VEC> us(p.u, p.u_bs, p.u_ts, x.b, row0), ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0),
         gs(p.dy, (long)p.T * p.C, p.C, x.b, row0);
     const unsigned ostep = (unsigned)p.C * (unsigned)sizeof(T);
@@ -532,7 +565,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
         gs.load(rg, el, d0, first, p.T);
         if (HASZ) zs.load(rz, el, d0, first, p.T);
     };
-    if (AHEAD) load(x.tile1 - 1);
+    if (AHEAD) load(max(x.end - 1, 0));
     float A2[NB], c[NB], dA[NB];
     auto load_A = [&](int sb) __attribute__((always_inline)) {
 #pragma unroll
@@ -548,10 +581,12 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int n = w * NS + sb * NB + j;
-            c[j] = p.dlast && n < p.N && x.ok ? p.dlast[((size_t)x.b * p.C + d) * p.N + n] : 0.f;
-            dA[j] = 0.f;
+            c[j] = dA[j] = 0.f;
+            if (n < p.N && x.ok) {
+                if (q.chunks > 1) c[j] = p.ends[(((size_t)x.b * q.chunks + x.chunk) * q.NP + n) * p.C + d];
+                else if (p.dlast) c[j] = p.dlast[((size_t)x.b * p.C + d) * p.N + n];
+            }
         }
-        chain<NB>(c, A2, p.ends, p.ends_step, q, p.C, x.b, w * NS + sb * NB, d, q.chunks - 1, -1, q.chunks - 1 - x.chunk);
         if (SB > 1) {
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
@@ -562,7 +597,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
     }
     // what only a tile's end needs is read again from the kernel's arguments there: kept over the loop it costs the scalar registers of B and C
     const __attribute__((address_space(4))) BwdArgs* args = (const __attribute__((address_space(4))) BwdArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-    for (int tile = x.tile1 - 1; tile >= x.tile0; --tile) {
+    for (int tile = x.end - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
         float cu[4], cslope[4], cz[4], csig[4], cdy[4], cstep[4], cg[4], su[4], h0[NB];
         if (!AHEAD) load(tile);
@@ -743,6 +778,21 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
         }
         // (no barrier: what the next tile writes before its first one is read here by nobody but its writer, or before the one above)
     }
+    if (x.end < x.tile1) {  // tiles behind the item's end: no gradient
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        const int slab = (blockIdx.x % q.nCb) % q.cbg;
+        asm volatile("" : "+s"(args));
+        const auto& pc = args->p;
+        for (int tile = x.end; tile < x.tile1; ++tile) {
+            const int first = tile * TS + w * RPW;
+            const size_t o = ((size_t)x.b * pc.T + first) * ostep;
+            store_elems<T>((char*)pc.du + o, ostep, el, d0, first, pc.T, zero);
+            store_elems<T>((char*)pc.ddelta + o, ostep, el, d0, first, pc.T, zero);
+            if (HASZ) store_elems<T>((char*)pc.dz + o, ostep, el, d0, first, pc.T, zero);
+            float* mo = pc.dmaps + ((size_t)slab * pc.B * pc.G * q.tiles + x.item + tile) * (4 * TS * 2 * NS);
+            for (int i = threadIdx.x; i < 4 * TS * 2 * NS; i += 256) mo[i] = 0.f;
+        }
+    }
     const size_t e = (size_t)x.b * q.chunks + x.chunk;
 #pragma unroll
     for (int sb = 0; sb < SB; ++sb) {
@@ -851,7 +901,7 @@ int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
     if (B < 1 || T < 1 || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
+    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 255) / 256 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
 }
 
@@ -866,12 +916,19 @@ int grid_for(size_t n) {
     return (int)(g < 4096 ? g : 4096);
 }
 
+int launch_carry(const float* A, const float* first, float* ends, const float* ends_step, const Plan& q, int B, int C, int N, int dir, hipStream_t s) {
+    scan_carry_kernel<<<(unsigned)(((size_t)B * N * C + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
+    GA_CHECK_LAUNCH();
+    return GA_OK;
+}
+
 template <typename T, int NS, bool HASZ, bool VEC>
 int launch_fwd_as(const Args& a, hipStream_t s) {
     const long blocks = (long)a.p.B * a.q.nCb;
     if (a.q.chunks > 1) {
         scan_fwd_kernel<T, NS, true, false, VEC><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
+        if (const int rc = launch_carry(a.p.A, a.p.state, a.p.ends, a.p.ends_step, a.q, a.p.B, a.p.C, a.p.N, 1, s)) return rc;
     }
     scan_fwd_kernel<T, NS, false, HASZ, VEC><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
@@ -889,6 +946,7 @@ int launch_bwd_as(const BwdArgs& a, hipStream_t s) {
     if (a.q.chunks > 1) {
         scan_bwd_ends_kernel<T, NS, HASZ, VEC><<<(unsigned)(blocks * (a.q.chunks - 1)), 256, 0, s>>>(a);
         GA_CHECK_LAUNCH();
+        if (const int rc = launch_carry(a.p.A, a.p.dlast, a.p.ends, a.p.ends_step, a.q, a.p.B, a.p.C, a.p.N, -1, s)) return rc;
     }
     scan_bwd_kernel<T, NS, HASZ, VEC><<<(unsigned)(blocks * a.q.chunks), 256, 0, s>>>(a);
     GA_CHECK_LAUNCH();
