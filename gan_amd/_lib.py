@@ -266,7 +266,7 @@ _ERR = {1: "GA_ERR_ARG (bad shape / unsupported configuration)", 2: "GA_ERR_LAUN
         3: "GA_ERR_ALIGN (pointer alignment)", 4: "GA_ERR_UNSUPPORTED (this variant does not take the shape)",
         5: "GA_ERR_SCRATCH (problem larger than the library's fixed split-K scratch: use ga_conv with a workspace)"}
 SPLITK_STATIC_FLOATS = 8 << 20
-CCONV_MAX_TAPS, SCAN_MAX_STATES, BNORM_MAX_C = 8, 64, 4096
+CCONV_MAX_TAPS, SCAN_MAX_STATES, SCAN_MAX_STRIDE, BNORM_MAX_C = 8, 64, (1 << 22) - 1, 4096
 
 
 def check(rc: int, what: str) -> None:

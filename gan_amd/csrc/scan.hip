@@ -850,50 +850,57 @@ __global__ __launch_bounds__(1024) void scan_dparams_kernel(const float* __restr
     }
 }
 
-// One token: a thread holds four states of a channel, TPC threads (a power of two) a channel; the state is read and written once.
+// One token: a thread holds four states of a channel, 1 << shift threads a channel, a block channels of one item (nb blocks an item); the state is
+// read and written once, and everything else is small.  Addresses are 32-bit offsets from scalar bases.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, int tpc) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, ch = i / tpc;
-    const int part = (int)(i % tpc), n0 = part * 4;
-    const bool ok = ch < (size_t)p.B * p.C;
-    const int b = ok ? (int)(ch / p.C) : 0, d = ok ? (int)(ch % p.C) : 0, g = d / (p.C / p.G);
-    const float u = (float)((const T*)p.u)[(size_t)b * p.u_bs + d];
-    const float raw = (float)((const T*)p.delta)[(size_t)b * p.delta_bs + d] + (p.delta_bias ? p.delta_bias[d] : 0.f);
-    const float step = p.softplus ? sq_softplus(raw) : raw;
-    float* hp = p.state + (size_t)b * p.state_bs + (size_t)d * p.N + n0;
-    const float* Ap = p.A + (size_t)d * p.N + n0;
-    const T* Bp = (const T*)p.Bm + (size_t)b * p.b_bs + (size_t)g * p.N + n0;
-    const T* Cp = (const T*)p.Cm + (size_t)b * p.c_bs + (size_t)g * p.N + n0;
-    float y = 0.f;
-    if (ok && n0 < p.N) {
-        float h[4], A[4];
-        if (VEC) {
-            *(float4*)h = *(const float4*)hp;
-            *(float4*)A = *(const float4*)Ap;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                h[j] = n0 + j < p.N ? hp[j] : 0.f;
-                A[j] = n0 + j < p.N ? Ap[j] : 0.f;
-            }
-        }
+__global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, int shift, unsigned nb) {
+    const unsigned b = blockIdx.x / nb, d = (blockIdx.x % nb) * (256u >> shift) + (threadIdx.x >> shift);
+    const int n0 = (int)(threadIdx.x & ((1u << shift) - 1)) * 4;
+    const unsigned dd = min(d, (unsigned)p.C - 1), g = p.G == 1 ? 0 : dd / (unsigned)(p.C / p.G);
+    const bool ok = d < (unsigned)p.C, mine = ok && n0 < p.N;
+    float* const state = p.state + (size_t)b * p.state_bs;
+    const T* const Bp = (const T*)p.Bm + (size_t)b * p.b_bs;
+    const T* const Cp = (const T*)p.Cm + (size_t)b * p.c_bs;
+    float h[4], A[4];
+    Quad<T> Bv, Cv;
+    if (VEC) {
+        const unsigned n = (unsigned)min(n0, p.N - 4);
+        *(float4*)h = *(const float4*)(state + (size_t)dd * p.N + n);
+        *(float4*)A = *(const float4*)(p.A + (size_t)dd * p.N + n);
+        Bv = *(const Quad<T>*)(Bp + g * p.N + n);
+        Cv = *(const Quad<T>*)(Cp + g * p.N + n);
+    } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (!VEC && n0 + j >= p.N) break;
-            h[j] = fmaf(__builtin_amdgcn_exp2f(step * (A[j] * SQ_LOG2E)), h[j], step * u * (float)Bp[j]);
-            y = fmaf((float)Cp[j], h[j], y);
+            const unsigned n = (unsigned)min(n0 + j, p.N - 1);
+            h[j] = state[(size_t)dd * p.N + n];
+            A[j] = p.A[(size_t)dd * p.N + n];
+            Bv.v[j] = Bp[(size_t)g * p.N + n];
+            Cv.v[j] = Cp[(size_t)g * p.N + n];
         }
-        if (VEC) *(float4*)hp = *(float4*)h;
+    }
+    const float u = (float)((const T*)p.u + (size_t)b * p.u_bs)[dd];
+    const float z = p.z ? (float)((const T*)p.z + (size_t)b * p.z_bs)[dd] : 0.f, D = p.D ? p.D[dd] : 0.f;
+    const float raw = (float)((const T*)p.delta + (size_t)b * p.delta_bs)[dd] + (p.delta_bias ? p.delta_bias[dd] : 0.f);
+    const float step = p.softplus ? sq_softplus(raw) : raw, su = step * u;
+    float y = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        h[j] = fmaf(__builtin_amdgcn_exp2f(step * (A[j] * SQ_LOG2E)), h[j], su * (float)Bv.v[j]);
+        if (mine && (VEC || n0 + j < p.N)) y = fmaf((float)Cv.v[j], h[j], y);
+    }
+    if (mine) {
+        if (VEC) *(float4*)(state + (size_t)d * p.N + n0) = *(float4*)h;
         else
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (n0 + j < p.N) hp[j] = h[j];
+                if (n0 + j < p.N) state[(size_t)d * p.N + n0 + j] = h[j];
     }
-    for (int o = tpc >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
-    if (ok && part == 0) {
-        if (p.D) y = fmaf(p.D[d], u, y);
-        if (p.z) y *= sq_silu((float)((const T*)p.z)[(size_t)b * p.z_bs + d]);
-        ((T*)p.y)[(size_t)b * p.C + d] = (T)y;
+    for (int o = 1 << shift >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
+    if (mine && n0 == 0) {
+        y = fmaf(D, u, y);
+        if (p.z) y *= sq_silu(z);
+        ((T*)p.y + (size_t)b * p.C)[d] = (T)y;
     }
 }
 
@@ -1041,17 +1048,18 @@ int ga_scan_step(const ga_scan_step_params* hp, int dtype, hipStream_t s) {
     const int rc = bad_sizes(p.B, 1, p.C, p.N, p.G, dtype);
     if (rc) return rc;
     if (!p.u || !p.delta || !p.A || !p.Bm || !p.Cm || !p.state || !p.y) return GA_ERR_ARG;
-    int tpc = 1;
-    while (tpc * 4 < p.N) tpc *= 2;
-    const size_t blocks = ((size_t)p.B * p.C * tpc + 255) / 256;
+    int shift = 0;
+    while ((4 << shift) < p.N) ++shift;
+    const size_t nb = ((size_t)p.C + (256 >> shift) - 1) / (256 >> shift), blocks = nb * p.B;
     if (blocks > 0x7fffffffUL) return GA_ERR_ARG;
-    const bool vec = p.N % 4 == 0 && p.state_bs % 4 == 0 && !(((uintptr_t)p.state | (uintptr_t)p.A) & 15);
+    const bool vec = p.N % 4 == 0 && p.state_bs % 4 == 0 && p.b_bs % 4 == 0 && p.c_bs % 4 == 0 && !(((uintptr_t)p.state | (uintptr_t)p.A) & 15) &&
+                     !(((uintptr_t)p.Bm | (uintptr_t)p.Cm) & (dtype == GA_DTYPE_BF16 ? 7 : 15));
     if (dtype == GA_DTYPE_BF16) {
-        if (vec) scan_step_kernel<bf16_t, true><<<(unsigned)blocks, 256, 0, s>>>(p, tpc);
-        else scan_step_kernel<bf16_t, false><<<(unsigned)blocks, 256, 0, s>>>(p, tpc);
+        if (vec) scan_step_kernel<bf16_t, true><<<(unsigned)blocks, 256, 0, s>>>(p, shift, (unsigned)nb);
+        else scan_step_kernel<bf16_t, false><<<(unsigned)blocks, 256, 0, s>>>(p, shift, (unsigned)nb);
     } else {
-        if (vec) scan_step_kernel<float, true><<<(unsigned)blocks, 256, 0, s>>>(p, tpc);
-        else scan_step_kernel<float, false><<<(unsigned)blocks, 256, 0, s>>>(p, tpc);
+        if (vec) scan_step_kernel<float, true><<<(unsigned)blocks, 256, 0, s>>>(p, shift, (unsigned)nb);
+        else scan_step_kernel<float, false><<<(unsigned)blocks, 256, 0, s>>>(p, shift, (unsigned)nb);
     }
     GA_CHECK_LAUNCH();
     return GA_OK;

@@ -13,14 +13,14 @@ __device__ __forceinline__ float sq_silu_slope(float x) {
 }
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|).  e: exp2 of the rounded product t = -|x| log2(e), times 1 + r with r = what t lacks
 // (without it e is off by |x| 2^-24 of itself: 4e-7 at the arguments of small step sizes).  log1p(e) = log(w) + (e - (w - 1)) / w with
-// w = fl(1 + e): the second term gives back what the sum lost, so that small results keep all their digits.  max(x, 0) as (x + |x|) / 2, which
-// passes a NaN on.  `sigmoid`: the slope, 1 / (1 + exp(-x)), from the same e and w.
+// w = fl(1 + e): the second term gives back what the sum lost, so that small results keep all their digits.  max(x, 0) as a choice that passes
+// a NaN on and gives 0 at minus infinity.  `sigmoid`: the slope, 1 / (1 + exp(-x)), from the same e and w.
 __device__ __forceinline__ float sq_softplus(float x, float& sigmoid) {
     const float ax = fminf(fabsf(x), 100.f), t = -ax * SQ_LOG2E;
     const float r = fmaf(-t, -1.9046542e-9f, fmaf(-t, SQ_LN2, -ax));  // ln 2 = fp32(ln 2) - 1.9046542e-9
     const float e2 = __builtin_amdgcn_exp2f(t), e = fmaf(e2, r, e2), w = 1.f + e, rw = __builtin_amdgcn_rcpf(w);
     sigmoid = (x < 0.f ? e : 1.f) * rw;
-    return fmaf(0.5f, x + fabsf(x), fmaf(__builtin_amdgcn_logf(w), SQ_LN2, (e - (w - 1.f)) * rw));
+    return (x < 0.f ? 0.f : x) + fmaf(__builtin_amdgcn_logf(w), SQ_LN2, (e - (w - 1.f)) * rw);
 }
 __device__ __forceinline__ float sq_softplus(float x) {
     float s;

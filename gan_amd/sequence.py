@@ -97,6 +97,12 @@ def _no_grad_step(name: str, whole: str, *ts) -> None:
         raise RuntimeError(f"{name} updates its state in place and has no gradient: call it under torch.no_grad(), or use {whole}")
 
 
+def _moved_on(state: Tensor) -> None:
+    """A state was written in place: a graph that had saved it refuses to go backwards through the new values."""
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+
+
 def _state_rows(name: str, t: Tensor, inner: int) -> int:
     """The batch stride of a state that a step updates in place: any, as long as its items are packed and apart."""
     want, n = [], 1
@@ -113,8 +119,8 @@ def _state_rows(name: str, t: Tensor, inner: int) -> int:
 def _conv_fwd(x, weight, bias, act, state, lengths, want_last):
     B, T, Cn = x.shape
     K = weight.shape[1]
-    y = torch.empty((B, T, Cn), device=x.device, dtype=x.dtype)
-    last = torch.empty((B, K - 1, Cn), device=x.device, dtype=x.dtype) if want_last else None
+    y = x.new_empty(B, T, Cn)
+    last = x.new_empty(B, K - 1, Cn) if want_last else None
     p = L.CausalConvParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), y.data_ptr(),
                            L.ptr(last) if K > 1 else 0, x.stride(0), x.stride(1), B, T, Cn, K, act)
     _call("ga_causal_conv_fwd", x.device, C.byref(p), L.dt(x))
@@ -137,18 +143,17 @@ class _CausalConv(torch.autograd.Function):
             return (None,) * 7
         B, T, Cn = x.shape
         K = weight.shape[1]
-        dev = x.device
-        dy = torch.zeros((B, T, Cn), device=dev, dtype=x.dtype) if dy is None else dy.contiguous()
+        dy = x.new_zeros(B, T, Cn) if dy is None else dy.contiguous()
         dlast = None if dlast is None or K == 1 else dlast.contiguous()
-        dx = torch.empty((B, T, Cn), device=dev, dtype=x.dtype)
+        dx = x.new_empty(B, T, Cn)
         dstate = torch.empty_like(state) if state is not None else None
-        dw = torch.empty((Cn, K), device=dev, dtype=torch.float32)
-        db = torch.empty((Cn,), device=dev, dtype=torch.float32) if bias is not None else None
-        ws = torch.empty((L.lib().ga_causal_conv_bwd_ws_elems(B, T, Cn, K),), device=dev, dtype=torch.float32)
+        dw = weight.new_empty(Cn, K)
+        db = weight.new_empty(Cn) if bias is not None else None
+        ws = weight.new_empty(L.lib().ga_causal_conv_bwd_ws_elems(B, T, Cn, K))
         p = L.CausalConvBwdParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), dy.data_ptr(),
                                   L.ptr(dlast), dx.data_ptr(), L.ptr(dstate) if K > 1 else 0, dw.data_ptr(), L.ptr(db), ws.data_ptr(),
                                   x.stride(0), x.stride(1), B, T, Cn, K, ctx.act)
-        _call("ga_causal_conv_bwd", dev, C.byref(p), L.dt(x))
+        _call("ga_causal_conv_bwd", x.device, C.byref(p), L.dt(x))
         return dx, dw, db, dstate, None, None, None
 
 
@@ -209,10 +214,11 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     _no_grad_step("causal_conv_step", "causal_conv", x, weight, bias, state)
     _one_device(x, weight, bias, state)
     x, weight, bias = _rows(x), _packed(weight), _packed(bias)
-    y = torch.empty((B, Cn), device=x.device, dtype=x.dtype)
+    y = x.new_empty(B, Cn)
     p = L.CausalConvStepParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), state.data_ptr() if K > 1 else 0, y.data_ptr(), x.stride(0), bs, B, Cn,
                                K, act)
     _call("ga_causal_conv_step", x.device, C.byref(p), dt)
+    _moved_on(state)
     return y
 
 
@@ -225,28 +231,23 @@ def _scan_sizes(B, T, Cn, N, G):
     return tuple((n + 3) & ~3 for n in (s.maps, s.hs, s.ends, s.ends_step, s.dmaps, s.dparams))
 
 
-def _f32(n: int, dev) -> Tensor:
-    return torch.empty((n,), device=dev, dtype=torch.float32)
-
-
 def _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, softplus, state, lengths, want_last, want_hs):
     B, T, Cn = u.shape
     G, N = Bm.shape[2:]
-    dev = u.device
     n_maps, n_hs, n_ends, n_step, _, _ = _scan_sizes(B, T, Cn, N, G)
-    y = torch.empty((B, T, Cn), device=dev, dtype=u.dtype)
-    last = torch.empty((B, Cn, N), device=dev, dtype=torch.float32) if want_last else None
-    keep = _f32(n_maps + n_hs if want_hs else n_maps + n_ends + n_step, dev)  # maps and hs for the backward pass, or maps and what ends here
+    y = u.new_empty(B, T, Cn)
+    last = A.new_empty(B, Cn, N) if want_last else None
+    keep = A.new_empty(n_maps + n_hs if want_hs else n_maps + n_ends + n_step)  # maps and hs for the backward pass, or maps and what ends here
     maps = keep.data_ptr()
     hs = maps + 4 * n_maps if want_hs else 0
     ends = 0
     if n_ends:
-        tmp = _f32(n_ends + n_step, dev) if want_hs else None
+        tmp = A.new_empty(n_ends + n_step) if want_hs else None
         ends = maps + 4 * n_maps if tmp is None else tmp.data_ptr()
     p = L.ScanParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
                      L.ptr(state), L.ptr(lengths), y.data_ptr(), L.ptr(last), maps, hs, ends, ends + 4 * n_ends, *u.stride()[:2], *delta.stride()[:2],
                      *((0, 0) if z is None else z.stride()[:2]), *Bm.stride()[:2], *Cm.stride()[:2], B, T, Cn, N, G, softplus)
-    _call("ga_scan_fwd", dev, C.byref(p), L.dt(u))
+    _call("ga_scan_fwd", u.device, C.byref(p), L.dt(u))
     return y, last, keep
 
 
@@ -266,20 +267,20 @@ class _SelectiveScan(torch.autograd.Function):
         B, T, G, N, softplus, has_state = ctx.cfg
         if dy is None and dlast is None:
             return (None,) * 12
-        Cn, dev, dt = u.shape[2], u.device, u.dtype
-        dy = torch.zeros((B, T, Cn), device=dev, dtype=dt) if dy is None else dy.contiguous()
+        Cn = u.shape[2]
+        dy = u.new_zeros(B, T, Cn) if dy is None else dy.contiguous()
         dlast = _packed(dlast)
         n_maps, _, n_ends, n_step, n_dmaps, n_dparams = _scan_sizes(B, T, Cn, N, G)
-        du = torch.empty((B, T, Cn), device=dev, dtype=dt)
-        ddelta = torch.empty((B, T, Cn), device=dev, dtype=dt)
-        dz = torch.empty((B, T, Cn), device=dev, dtype=dt) if z is not None else None
-        dB = torch.empty((B, T, G, N), device=dev, dtype=dt)
-        dC = torch.empty((B, T, G, N), device=dev, dtype=dt)
-        dA = torch.empty((Cn, N), device=dev, dtype=torch.float32)
-        dD = _f32(Cn, dev) if D is not None else None
-        dbias = _f32(Cn, dev) if delta_bias is not None else None
-        dstate = torch.empty((B, Cn, N), device=dev, dtype=torch.float32) if has_state else None
-        ws = _f32(n_ends + n_step + n_dmaps + n_dparams, dev)
+        du = u.new_empty(B, T, Cn)
+        ddelta = u.new_empty(B, T, Cn)
+        dz = u.new_empty(B, T, Cn) if z is not None else None
+        dB = u.new_empty(B, T, G, N)
+        dC = u.new_empty(B, T, G, N)
+        dA = A.new_empty(Cn, N)
+        dD = A.new_empty(Cn) if D is not None else None
+        dbias = A.new_empty(Cn) if delta_bias is not None else None
+        dstate = A.new_empty(B, Cn, N) if has_state else None
+        ws = A.new_empty(n_ends + n_step + n_dmaps + n_dparams)
         ends = ws.data_ptr()
         step, maps = ends + 4 * n_ends, keep.data_ptr()
         dmaps = step + 4 * n_step
@@ -287,7 +288,7 @@ class _SelectiveScan(torch.autograd.Function):
                             L.ptr(dlast), maps, maps + 4 * n_maps, du.data_ptr(), ddelta.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr(),
                             dA.data_ptr(), L.ptr(dD), L.ptr(dbias), L.ptr(dstate), ends, step, dmaps, dmaps + 4 * n_dmaps, *u.stride()[:2],
                             *delta.stride()[:2], *((0, 0) if z is None else z.stride()[:2]), B, T, Cn, N, G, softplus)
-        _call("ga_scan_bwd", dev, C.byref(p), L.dt(u))
+        _call("ga_scan_bwd", u.device, C.byref(p), L.dt(u))
         return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None
 
 
@@ -304,9 +305,18 @@ def _scan_maps(name: str, t: Tensor, lead, Cn: int, dtype) -> Tensor:
     return t
 
 
+def _scan_rows(t: Optional[Tensor]) -> Optional[Tensor]:
+    """_rows, with rows no further apart than the kernels' 32-bit offsets go."""
+    if t is None or (t.stride(2) == 1 and t.stride(1) <= L.SCAN_MAX_STRIDE):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)  # (contiguous() leaves the stride of a single row as it is)
+
+
 def _scan_checks(u, delta, A, Bm, Cm, D, z, delta_bias, state):
     lead, Cn = u.shape[:-1], u.shape[-1]
     L.dt(u)
+    if Cn > L.SCAN_MAX_STRIDE:
+        raise ValueError(f"u: at most {L.SCAN_MAX_STRIDE} channels, got {Cn}")
     _act("delta", delta, u.shape, u.dtype)
     _act("z", z, u.shape, u.dtype)
     Bm, Cm = _scan_maps("Bm", Bm, lead, Cn, u.dtype), _scan_maps("Cm", Cm, lead, Cn, u.dtype)
@@ -337,7 +347,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Tensor, 
     Bm, Cm = _scan_checks(u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _lengths(lengths, u.shape[0])
     _one_device(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths)
-    u, delta, z, Bm, Cm = _rows(u), _rows(delta), _rows(z), _maps(Bm), _maps(Cm)
+    u, delta, z, Bm, Cm = _scan_rows(u), _scan_rows(delta), _scan_rows(z), _maps(Bm), _maps(Cm)
     A, D, delta_bias, state, lengths = _packed(A), _packed(D), _packed(delta_bias), _packed(state), _packed(lengths)
     if _wants_grad(u, delta, A, Bm, Cm, D, z, delta_bias, state):
         y, last = _SelectiveScan.apply(u, delta, A, Bm, Cm, D, z, delta_bias, state, int(bool(softplus)), lengths, bool(return_state))
@@ -361,11 +371,12 @@ def selective_scan_step(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Ten
     _no_grad_step("selective_scan_step", "selective_scan", u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _one_device(u, delta, A, Bm, Cm, D, z, delta_bias, state)
     u, delta, z, Bm, Cm, A, D, delta_bias = _rows(u), _rows(delta), _rows(z), _maps(Bm), _maps(Cm), _packed(A), _packed(D), _packed(delta_bias)
-    y = torch.empty((B, Cn), device=u.device, dtype=u.dtype)
+    y = u.new_empty(B, Cn)
     p = L.ScanStepParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
                          state.data_ptr(), y.data_ptr(), u.stride(0), delta.stride(0), 0 if z is None else z.stride(0), Bm.stride(0), Cm.stride(0), bs,
                          B, Cn, N, G, int(softplus))
     _call("ga_scan_step", u.device, C.byref(p), L.dt(u))
+    _moved_on(state)
     return y
 
 
@@ -376,13 +387,12 @@ def _gate_rows(gate: Optional[Tensor]) -> int:
 
 def _norm_fwd(x, branch, gate, w, b, wp, bp, scale, ab, post, layer, eps, dtype, want_stats):
     B, T, Cn = x.shape
-    dev = x.device
-    y = torch.empty((B, T, Cn), device=dev, dtype=dtype)
-    r = torch.empty((B, T, Cn), device=dev, dtype=x.dtype) if branch is not None else None
-    stats = torch.empty((B * T, 4), device=dev, dtype=torch.float32) if want_stats else None
+    y = x.new_empty((B, T, Cn), dtype=dtype)
+    r = x.new_empty(B, T, Cn) if branch is not None else None
+    stats = x.new_empty((B * T, 4), dtype=torch.float32) if want_stats else None
     p = L.BlockNormParams(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab), L.ptr(r),
                           y.data_ptr(), L.ptr(stats), B, T, Cn, int(post), int(layer), _gate_rows(gate), eps)
-    _call("ga_block_norm_fwd", dev, C.byref(p), L.dt(x), L.dt(y))
+    _call("ga_block_norm_fwd", x.device, C.byref(p), L.dt(x), L.dt(y))
     return r, y, stats
 
 
@@ -403,18 +413,16 @@ class _BlockNorm(torch.autograd.Function):
         if dr is None and dy is None:
             return (None,) * 13
         B, T, Cn = x.shape
-        dev = x.device
         dr, dy = _packed(dr), _packed(dy)
-        like = lambda t: torch.empty(t.shape, device=dev, dtype=t.dtype) if t is not None else None  # noqa: E731
-        dx = torch.empty((B, T, Cn), device=dev, dtype=x.dtype)
-        dbranch, dgate, dw, db, dwp, dbp, dscale, dab = (like(t) for t in (branch, gate, w, b, wp, bp, scale, ab))
+        dx, dbranch, dgate, dw, db, dwp, dbp, dscale, dab = (None if t is None else torch.empty_like(t)  # (all packed)
+                                                             for t in (x, branch, gate, w, b, wp, bp, scale, ab))
         rows = _gate_rows(gate)
         by_item = ab is not None or (gate is not None and not rows)
-        ws = torch.empty((L.lib().ga_block_norm_bwd_ws_elems(B, T, Cn, int(by_item)),), device=dev, dtype=torch.float32)
+        ws = stats.new_empty(L.lib().ga_block_norm_bwd_ws_elems(B, T, Cn, int(by_item)))
         p = L.BlockNormBwdParams(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab),
                                  stats.data_ptr(), L.ptr(dr), L.ptr(dy), dx.data_ptr(), L.ptr(dbranch), L.ptr(dgate), L.ptr(dw), L.ptr(db), L.ptr(dwp),
                                  L.ptr(dbp), L.ptr(dscale), L.ptr(dab), ws.data_ptr(), B, T, Cn, int(post), int(layer), rows)
-        _call("ga_block_norm_bwd", dev, C.byref(p), L.dt(x), L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F32)
+        _call("ga_block_norm_bwd", x.device, C.byref(p), L.dt(x), L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F32)
         return dx, dbranch, dgate, dw, db, dwp, dbp, dscale, dab, None, None, None, None
 
 
@@ -441,8 +449,8 @@ def block_norm(x: Tensor, branch: Optional[Tensor] = None, *, weight: Optional[T
     L.dt(x)
     if kind not in ("rms", "layer"):
         raise ValueError(f"kind: 'rms' or 'layer' expected, got {kind!r}")
-    if not eps > 0:
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not 1e-30 <= eps < float("inf"):
+        raise ValueError(f"eps: a positive number that float32 holds expected (1e-30 or more), got {eps}")
     if branch is None:
         if post_norm or post_weight is not None or post_bias is not None or gate is not None or scale is not None:
             raise ValueError("post_norm, post_weight, post_bias, gate and scale belong to a branch")

@@ -604,3 +604,111 @@ def test_more_than_two_to_the_31_elements():
     # one item alone is cut into chunks, the large batch is not: the states differ by float32 roundings, the outputs by a bf16 step at most
     assert float((y[-1:].float() - y1.float()).abs().max()) <= 2 ** -7 * float(y1.float().abs().max())
     assert bool((y[0] == y[1]).all())
+
+
+# ------------------------------------------------------------------------------------------------ calls that the lists above leave out
+SCAN_CHUNKS = [  # as SCAN: many chunks in time, items that end chunks before the last row, every number of states a wave can hold
+    (6, 700, 40, 16, 1, F32, True, True, True, True, True, True),
+    (6, 333, 72, 12, 2, BF, True, True, True, True, True, True),
+    (1, 4500, 12, 4, 1, F32, False, True, True, True, True, False),  # more tiles than chunks
+    (2, 300, 70, 64, 1, F32, True, True, True, True, True, True),
+    (3, 210, 68, 32, 1, BF, True, True, False, True, True, False),
+]
+
+
+@pytest.mark.parametrize("case", SCAN_CHUNKS, ids=str)
+def test_selective_scan_in_many_chunks(case):
+    test_selective_scan_and_its_gradients(case)
+
+
+def test_selective_scan_of_rows_far_apart():
+    """Rows further apart than the kernels' offsets reach are copied; so is a single row with a stride that nothing uses."""
+    B, T, C, N = 2, 3, 40, 5
+    g = gen(31)
+    A, Bm, Cm = -rnd(g, C, N).abs() - 0.1, rnd(g, B, T, N), rnd(g, B, T, N)
+    far = torch.zeros(B * T, L.SCAN_MAX_STRIDE + 9, device=DEV)
+    u = far.view(B, T, -1)[..., 3:C + 3]
+    u.copy_(rnd(g, B, T, C))
+    leaf = u.detach().requires_grad_()
+    packed = u.contiguous().requires_grad_()
+    dy = rnd(g, B, T, C)
+    y, y2 = (S.selective_scan(t, t, A, Bm, Cm, z=t) for t in (leaf, packed))
+    assert torch.equal(y, y2)
+    got, want = (torch.autograd.grad(o, t, dy)[0] for o, t in ((y, leaf), (y2, packed)))
+    # the three gradients of the one leaf (as u, delta and z) are added up in autograd's order, which the copies change: either order makes two
+    # roundings of partial sums that are at most |p1| + |p2| + |p3|, so the two differ by at most 4 * 2^-24 of it (and one rounding of the bound)
+    apart = [packed.detach().clone().requires_grad_() for _ in range(3)]
+    parts = torch.autograd.grad(S.selective_scan(apart[0], apart[1], A, Bm, Cm, z=apart[2]), apart, dy)
+    assert bool(((got - want).abs() <= 4.01 * 2.0 ** -24 * sum(p.abs() for p in parts)).all())
+    one = u[:, :1].as_strided((B, 1, C), (u.stride(0), 1 << 40, 1), u.storage_offset())
+    want = S.selective_scan(packed[:, :1].detach(), packed[:, :1].detach(), A, Bm[:, :1], Cm[:, :1])
+    assert torch.equal(S.selective_scan(one, one, A, Bm[:, :1], Cm[:, :1]), want)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("value", ["-inf", "lowest"])
+def test_rows_masked_through_their_step(dt, value):
+    """delta = minus infinity, or the type's lowest value, is a step of zero: the row leaves the states alone and gets no gradient through it
+    (the reference gets -1e4, whose exp is zero in 64 bits too)."""
+    case = (2, 45, 68, 16, 1, dt, True, True, True, True, True, False)
+    a, _, dy, dl = make_scan(case)
+    cut = float("-inf") if value == "-inf" else torch.finfo(dt).min
+    rows = torch.zeros(45, dtype=torch.bool, device=DEV)
+    rows[5:9] = rows[16:33] = True
+    leaves = {k: v.detach().clone() for k, v in a.items()}
+    leaves["delta"][:, rows] = cut
+    a["delta"] = a["delta"].clone()
+    a["delta"][:, rows] = -1e4
+    for v in leaves.values():
+        v.requires_grad_(True)
+    y, last = S.selective_scan(**leaves, return_state=True)
+    got = dict(zip(leaves, grads([y, last], list(leaves.values()), [dy, dl])))
+    ref = R.scan(**a, softplus=True, lengths=None, dy=dy, dlast=dl)
+    assert float(got["delta"][:, rows].float().abs().max()) <= 1e-37
+    for name, t in (("y", y), ("last", last), *got.items()):
+        if name != "delta":
+            R.close(t, *ref[name], k_scan(*case[:5]), name)
+    with torch.no_grad():
+        st = leaves["state"].detach().clone()
+        row = {k: (v[:, 5].detach() if v.dim() > 2 else v.detach()) for k, v in leaves.items() if k != "state"}
+        S.selective_scan_step(**row, state=st)
+        assert torch.equal(st, leaves["state"])
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_selective_scan_step_reads_slices_in_place(dt):
+    """Offsets and strides that leave no vector access, and one that leaves it to the state alone: the same bits as packed tensors."""
+    B, C, N, G = 5, 70, 12, 2
+    g = gen(41)
+    wide, maps = rnd(g, B, 3 * C + 1, dtype=dt), rnd(g, B, 1 + 2 * G * N, dtype=dt)
+    u, delta, z = wide[:, 1:C + 1], wide[:, C + 1:2 * C + 1], wide[:, 2 * C + 1:]
+    Bm, Cm = maps[:, 1:G * N + 1].unflatten(1, (G, N)), maps[:, G * N + 1:].unflatten(1, (G, N))
+    A, D, state = -rnd(g, C, N).abs(), rnd(g, C), rnd(g, B, C, N)
+    want_state = state.clone()
+    want = S.selective_scan_step(u.contiguous(), delta.contiguous(), A, Bm.contiguous(), Cm.contiguous(), want_state, D=D, z=z.contiguous())
+    odd = torch.empty(B * C * N + 1, device=DEV)[1:].view(B, C, N)
+    apart = torch.empty(B, C * N + 3, device=DEV)[:, :C * N].unflatten(1, (C, N))
+    for st in (state.clone(), odd, apart):
+        st.copy_(state)
+        assert torch.equal(S.selective_scan_step(u, delta, A, Bm, Cm, st, D=D, z=z), want) and torch.equal(st, want_state)
+
+
+def test_a_graph_that_saved_a_state_refuses_it_after_a_step():
+    g = gen(51)
+    x, w, st = rnd(g, 2, 6, 8).requires_grad_(), rnd(g, 8, 4), rnd(g, 2, 3, 8)
+    y = S.causal_conv(x, w.requires_grad_(), state=st)
+    with torch.no_grad():
+        S.causal_conv_step(x[:, 0], st, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    h = rnd(g, 2, 8, 3)
+    q = rnd(g, 2, 8, 3).requires_grad_()
+    prod = q * h
+    with torch.no_grad():
+        S.selective_scan_step(x[:, 0], x[:, 1], -w[:, :3].abs(), w[:2, :3].contiguous(), w[2:4, :3].contiguous(), h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        prod.sum().backward()
+    with torch.inference_mode():
+        h2 = torch.zeros(2, 8, 3, device=DEV)
+        S.selective_scan_step(x[:, 0], x[:, 1], -w[:, :3].abs(), w[:2, :3].contiguous(), w[2:4, :3].contiguous(), h2)
+        assert bool((h2 != 0).any())

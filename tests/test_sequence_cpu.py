@@ -201,3 +201,16 @@ def test_c_entries_refuse_bad_sizes_without_a_launch():
     assert lib.ga_block_norm_bwd(C.byref(L.BlockNormBwdParams(B=1, T=1, C=8)), 0, 0, None) == 1
     assert lib.ga_causal_conv_bwd_ws_elems(1, 1, 8, 9) == 0 and lib.ga_causal_conv_bwd_ws_elems(2, 40, 8, 4) > 0
     assert lib.ga_block_norm_bwd_ws_elems(1, 1, 9000, 0) == 0 and lib.ga_block_norm_bwd_ws_elems(3, 5, 8, 1) >= (3 + 3) * 4 * 8
+
+
+@pytest.mark.parametrize("eps", [float("nan"), float("inf"), -1e-6, 1e-46])
+def test_block_norm_refuses_an_eps_that_float32_does_not_hold(eps):
+    with pytest.raises(ValueError, match="eps"):
+        S.block_norm(rnd(2, 5, 8), eps=eps)
+
+
+def test_selective_scan_refuses_more_channels_than_its_offsets_reach():
+    Cn = L.SCAN_MAX_STRIDE + 1
+    u = torch.zeros(1).expand(1, 1, Cn)
+    with pytest.raises(ValueError, match="channels"):
+        S.selective_scan(u, u, torch.zeros(1, 1).expand(Cn, 1), torch.zeros(1, 1, 1), torch.zeros(1, 1, 1))
