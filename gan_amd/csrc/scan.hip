@@ -221,35 +221,51 @@ __device__ __forceinline__ void get_sum2(float (&x)[4], float (&y)[4], float2 (*
 }
 
 // What comes into each chunk, from what each one leaves behind by itself, in place: carry' = exp(A sum of steps) carry + end, over the chunks
-// in order (forward) or against it (backward: dir < 0), from `first` [B][C][N] (or zero).  A thread is one state of one channel, with the loads
-// of 32 chunks in flight: few threads, a long way to memory.  (As a loop at the start of every block of the main kernel it cost 11 of the 23 us
-// that a prompt of 2250 rows and 8 blocks spent there.)
-__global__ __launch_bounds__(256) void scan_carry_kernel(const float* __restrict__ A, const float* __restrict__ first, float* __restrict__ ends,
-                                                         const float* __restrict__ ends_step, Plan q, int B, int C, int N, int dir) {
-    constexpr int U = 32;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)B * N * C) return;
+// in order (forward) or against it (backward: dir < 0), from `first` [B][C][N] (or zero).  A wave takes 64 states and one of SEGS runs of up to U
+// chunks, all their loads in flight at once (few threads, a long way to memory); with more runs than one each is first walked from zero, and the
+// runs' ends meet in LDS.  (As a loop at the start of every block of the main kernel it cost 11 of the 23 us that a prompt of 2250 rows and 8
+// blocks spent there; as a kernel that walks 71 chunks in one run, 11 us.)
+template <int SEGS, int U>
+__global__ __launch_bounds__(SEGS > 1 ? SEGS * 64 : 256) void scan_carry_kernel(const float* __restrict__ A, const float* __restrict__ first,
+                                                                               float* __restrict__ ends, const float* __restrict__ ends_step, Plan q,
+                                                                               int B, int C, int N, int dir) {
+    __shared__ float se[SEGS][64], st[SEGS][64];
+    const int lane = threadIdx.x & 63, seg = SEGS > 1 ? threadIdx.x >> 6 : 0;
+    const size_t id = SEGS > 1 ? (size_t)blockIdx.x * 64 + lane : (size_t)blockIdx.x * 256 + threadIdx.x, all = (size_t)B * N * C;
+    const size_t i = id < all ? id : all - 1;
     const int d = (int)(i % C), n = (int)(i / C % N), b = (int)(i / C / N);
+    const int run = (q.chunks + SEGS - 1) / SEGS, k0 = seg * run, k1 = min(k0 + run, q.chunks);  // (run <= U)
     const float A2 = A[(size_t)d * N + n] * SQ_LOG2E;
     float c = first ? first[((size_t)b * C + d) * N + n] : 0.f;
     const float* sp = ends_step + (size_t)b * q.chunks * C + d;
     float* ep = ends + ((size_t)b * q.chunks * q.NP + n) * C + d;
-    for (int k = 0; k < q.chunks; k += U) {
-        float sum[U], end[U];
+    float sum[U], end[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kk = min(k + u, q.chunks - 1), chunk = dir < 0 ? q.chunks - 1 - kk : kk;
-            sum[u] = sp[(size_t)chunk * C];
-            end[u] = ep[(size_t)chunk * q.NP * C];
-        }
+    for (int u = 0; u < U; ++u) {
+        const int k = min(k0 + u, q.chunks - 1), chunk = dir < 0 ? q.chunks - 1 - k : k;
+        sum[u] = sp[(size_t)chunk * C];
+        end[u] = ep[(size_t)chunk * q.NP * C];
+    }
+    if (SEGS > 1) {
+        float total = 0.f, e = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (k + u < q.chunks) {
-                const int chunk = dir < 0 ? q.chunks - 1 - (k + u) : k + u;
-                ep[(size_t)chunk * q.NP * C] = c;
-                c = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), c, end[u]);  // (of the last chunk: not written by any block, not used)
+            if (k0 + u < k1) {
+                e = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), e, end[u]);
+                total += sum[u];
             }
+        se[seg][lane] = e;
+        st[seg][lane] = total;
+        __syncthreads();
+        for (int j = 0; j < seg; ++j) c = fmaf(__builtin_amdgcn_exp2f(st[j][lane] * A2), c, se[j][lane]);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (k0 + u < k1 && id < all) {
+            const int chunk = dir < 0 ? q.chunks - 1 - (k0 + u) : k0 + u;
+            ep[(size_t)chunk * q.NP * C] = c;
+            c = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), c, end[u]);  // (what the last chunk leaves is written by no block, and used here by nobody)
+        }
 }
 
 // ENDS: only the state that each chunk but the last leaves behind when it starts from zero, and the sum of its steps
@@ -908,7 +924,7 @@ int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
     if (B < 1 || T < 1 || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 255) / 256 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
+    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 63) / 64 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
 }
 
@@ -924,7 +940,11 @@ int grid_for(size_t n) {
 }
 
 int launch_carry(const float* A, const float* first, float* ends, const float* ends_step, const Plan& q, int B, int C, int N, int dir, hipStream_t s) {
-    scan_carry_kernel<<<(unsigned)(((size_t)B * N * C + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
+    const size_t states = (size_t)B * N * C;
+    static_assert(MAX_CHUNKS <= 16 * 16, "runs of the carry kernel");
+    if (q.chunks <= 8) scan_carry_kernel<1, 8><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
+    else if (q.chunks <= 32) scan_carry_kernel<1, 32><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
+    else scan_carry_kernel<16, 16><<<(unsigned)((states + 63) / 64), 1024, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }

@@ -105,6 +105,8 @@ def _moved_on(state: Tensor) -> None:
 
 def _state_rows(name: str, t: Tensor, inner: int) -> int:
     """The batch stride of a state that a step updates in place: any, as long as its items are packed and apart."""
+    if t.is_contiguous():
+        return inner
     want, n = [], 1
     for s in reversed(t.shape[1:]):
         want.append(n)
