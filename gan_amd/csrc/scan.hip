@@ -81,6 +81,12 @@ __global__ __launch_bounds__(256) void scan_maps_kernel(const T* __restrict__ Bm
     }
 }
 
+// The wave's part of a tile's B and C on its way from memory to this XCD's L2 while the rows come: the scalar loads of a tile follow one another, and
+// each would wait for memory by itself.  (One word of every 128 bytes or less; `arrived` keeps the load.)
+template <int NS>
+__device__ __forceinline__ float warm(const float* wave_maps, int lane) { return wave_maps[lane * (TS * 2 * NS) / 64]; }
+__device__ __forceinline__ void arrived(float v) { asm volatile("" ::"v"(v)); }
+
 // Where a block and a lane are.  `d` counts channels, unsigned so that an address is a scalar base plus a 32-bit offset.
 struct Place {
     int lane, w, chunk, b, g, len, tile0, tile1;
@@ -318,7 +324,9 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     const unsigned ystep = (unsigned)p.C * (unsigned)sizeof(T);
     char* yp = (char*)p.y + ((size_t)x.b * p.T + row0) * ystep;
     Quad<T> ru, rd, rz;
+    float wm;
     auto load = [&](int tile) __attribute__((always_inline)) {
+        wm = warm<NS>(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS), lane);
         us.load(ru, el, d0, tile * TS + w * RPW, p.T);
         ds.load(rd, el, d0, tile * TS + w * RPW, p.T);
         if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
@@ -336,6 +344,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Args a) {
     for (int tile = x.tile0; tile < x.end; ++tile) {
         float cu[4], cz[4], step[4], su[4];
         bool live[4];
+        arrived(wm);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             live[e] = el.ok() && tile * TS + el.row(e) < len;
@@ -460,7 +469,9 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     const int row0 = max(x.end - 1, 0) * TS + w * RPW;
     Rows<T, VEC> ds(p.delta, p.delta_bs, p.delta_ts, x.b, row0), zs(p.z, p.z_bs, p.z_ts, x.b, row0), gs(p.dy, (long)p.T * p.C, p.C, x.b, row0);
     Quad<T> rd, rz, rg;
+    float wm;
     auto load = [&](int tile) __attribute__((always_inline)) {
+        wm = warm<NS>(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS), lane);
         ds.load(rd, el, d0, tile * TS + w * RPW, p.T);
         gs.load(rg, el, d0, tile * TS + w * RPW, p.T);
         if (HASZ) zs.load(rz, el, d0, tile * TS + w * RPW, p.T);
@@ -477,6 +488,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(BwdArgs a) {
     for (int tile = x.end - 1; tile >= x.tile0; --tile) {
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
         float step[4], dy[4];
+        arrived(wm);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const bool live = el.ok() && tile * TS + el.row(e) < len;
@@ -573,7 +585,9 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
 #pragma unroll
         for (int j = 0; j < NB; ++j) hn[j] = at<float>(hp + (size_t)j * p.C, d);
     };
+    float wm;
     auto load = [&](int tile) __attribute__((always_inline)) {
+        if (AHEAD) wm = warm<NS>(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS), lane);
         load_h(tile, 0);
         const int first = tile * TS + w * RPW;
         us.load(ru, el, d0, first, p.T);
@@ -617,6 +631,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
         uniform_ptr mp = (uniform_ptr)(uintptr_t)(p.maps + ((x.item + tile) * 4 + w) * (TS * 2 * NS));
         float cu[4], cslope[4], cz[4], csig[4], cdy[4], cstep[4], cg[4], su[4], h0[NB];
         if (!AHEAD) load(tile);
+        if (AHEAD) arrived(wm);
         if (SB > 1) {
             const float* pb = p.delta_bias;
             asm volatile("" : "+s"(pb));  // (loaded here and not kept over the loop)
