@@ -6,6 +6,9 @@
 //
 // A row is held in the registers of 64 lanes (one wave) or of a whole block.  Column sums (the parameters' gradients) stay in registers over a
 // block's rows and leave as one row of partial sums per block, added up in a fixed order: results do not depend on timing.
+//
+// Measured at 16 x 2250 x 1024, residual float32, the rest bf16, a gate per row: forward 105 us (516 MB: 4.9 TB/s, what a large copy reaches),
+// backward 159 us (811 MB: 5.1 TB/s) and 10 us for the parameter sums.  64 x 375 x 512 bf16: 22 and 39 us; one row of 64 items: 5 us.
 #include "seq_common.h"
 
 namespace {
@@ -109,7 +112,9 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][P][V], float (&mea
     BN_ROWS rstd[j] = 1.f / sqrtf(fmaf(s[j], inv, eps));
 }
 
-// G threads a row, P pieces of V columns a thread, R rows at a time: their loads are in flight together and their sums share the exchanges
+// G threads a row, P pieces of V columns a thread, R rows at a time: their loads are in flight together and their sums share the exchanges.
+// (One row at a time against this: 16 x 2250 x 1024 102 + 173 against 105 + 169 us, 64 x 375 x 256 13.5 + 26.8 against 12.4 + 28.0; one row an
+// item 4.4 against 5.0.)
 template <typename TX, typename TO, int G, int P, int V, int R>
 __global__ __launch_bounds__(G == 64 ? 256 : G) void bnorm_fwd_kernel(ga_block_norm_params p, long rows_per_item, int parts) {
     BN_COLUMNS();
@@ -431,6 +436,9 @@ struct Bwd {
     }
 };
 
+// Quads of columns where the width and the bases allow (16 x 562 x 4096 bf16 58 + 121 us; single columns 62 + 126).  Up to 512 columns a row is a
+// wave's: 64 x 375 x 512 takes 22 + 39 us, and 34 + 58 with 256 threads a row, half of them idle.  A wave with 1024 columns does not fit the
+// registers (22 to 39 spilled in the backward kernel).
 template <typename TX, typename TO, typename F, typename A>
 int by_width(const A& p, bool vec, F f) {
     if (vec) {

@@ -5,6 +5,15 @@
 // along time in tiles of 16 rows.  What depends on a row and a channel alone (softplus, gates, the sums over states) is done once, four rows to
 // a wave, and passes through LDS; B and C, which all channels of a group share, are first laid out in float32 in the order in which
 // the waves read them (scan_maps_kernel) and come in as scalar loads, so that they cost no vector instruction and no LDS bandwidth.
+// Time is cut into chunks where channels and items alone do not fill the card: a first kernel walks every chunk from zero, a small one carries
+// the states from chunk to chunk, the main one then walks each chunk from the state that comes in.
+//
+// Bound by instruction issue: a state and row is a multiply and an exp2 for the decay, a multiply and two multiply-adds (exp2 alone takes the time
+// of two others), and walks through the first kernel (two thirds of it) as well.  At 16 x 2250 x 1024 with 16 states, bf16: forward 270 us
+// (first kernel 115, main 176; 227 MB, 46 us of memory time), with the saved states 275; backward 619 us (first 121, main 522, sums 28; the states
+// walked again, the adjoint, and sums over 64 channels for dB and dC).  12 x 375 x 512: 40 and 66 us; one prompt of 2250 x 512: 32 us.  8 states 187
+// and 405 us; half the items with 32 states 248 and 929 us (a wave's 8 states take turns, the rest waits in LDS, one block a CU); a quarter
+// with 64 states 243 and 831 us.
 #include "seq_common.h"
 
 namespace {
@@ -120,7 +129,7 @@ __device__ __forceinline__ T at(const void* base, unsigned d) { return *(const T
 
 template <typename T> struct alignas(4 * sizeof(T)) Quad { T v[4]; };
 
-// The four elements of a tile that a lane prepares and finishes.  VEC: four adjacent channels of one row, one access for all four rows of a wave;
+// The four elements of a tile that a lane prepares and finishes.  (16 x 2250 x 1024 x 16 bf16: 270 + 619 us; one channel at a time 276 + 725.)  VEC: four adjacent channels of one row, one access for all four rows of a wave;
 // otherwise (alignment, odd widths) one channel of each of the four rows.
 template <bool VEC>
 struct Elems {
@@ -550,7 +559,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int NB = NS < 4 ? NS : 4, SB = NS / NB, U = 2;
-    constexpr bool AHEAD = SB == 1 && VEC && sizeof(T) == 2;  // registers for the next tile's rows on their way
+    constexpr bool AHEAD = SB == 1 && VEC && sizeof(T) == 2;  // the next tile's rows on their way (float32 rows, or ones of single channels, spill)
     __shared__ __attribute__((aligned(16))) float2 sd[TS][64];     // step, step * u
     __shared__ __attribute__((aligned(16))) float sg[TS][64];      // dy * gate
     __shared__ __attribute__((aligned(16))) float sy[4][TS][64];   // <C, h> over a wave's states
@@ -882,7 +891,8 @@ __global__ __launch_bounds__(1024) void scan_dparams_kernel(const float* __restr
 }
 
 // One token: a thread holds four states of a channel, 1 << shift threads a channel, a block channels of one item (nb blocks an item); the state is
-// read and written once, and everything else is small.  Addresses are 32-bit offsets from scalar bases.
+// read and written once, and everything else is small: 256 x 1024 x 16 states, bf16, 7.8 us (35.7 MB: 4.6 TB/s), 17.5 with single elements of
+// state, A, B and C (odd N or unaligned bases); 256 x 1024 x 64 28 us; one item of 512 x 16 2.5 us.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, int shift, unsigned nb) {
     const unsigned b = blockIdx.x / nb, d = (blockIdx.x % nb) * (256u >> shift) + (threadIdx.x >> shift);
@@ -939,7 +949,8 @@ int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
     if (B < 1 || T < 1 || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 63) / 64 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL) return GA_ERR_ARG;
+    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 63) / 64 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL)
+        return GA_ERR_ARG;
     return GA_OK;
 }
 
@@ -957,6 +968,7 @@ int grid_for(size_t n) {
 int launch_carry(const float* A, const float* first, float* ends, const float* ends_step, const Plan& q, int B, int C, int N, int dir, hipStream_t s) {
     const size_t states = (size_t)B * N * C;
     static_assert(MAX_CHUNKS <= 16 * 16, "runs of the carry kernel");
+    // (8 chunks at 16 x 2250 x 1024: 5.6 us, 8.3 with loads for 32; 32 chunks at 4 x 2250 x 512: the whole forward pass 62 us, 67 with 16 runs)
     if (q.chunks <= 8) scan_carry_kernel<1, 8><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
     else if (q.chunks <= 32) scan_carry_kernel<1, 32><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
     else scan_carry_kernel<16, 16><<<(unsigned)((states + 63) / 64), 1024, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);

@@ -521,8 +521,8 @@ int ga_lstm_bwd(const ga_lstm_bwd_params* h_params, ga_stream_t stream);
 
 /* ---- sequence operators: linear-time mixing along time for models on codec latents, next to ga_conv / ga_lstm_* / ga_gn_* ----
  * No reference call site: they extend the operator set.  Element strides (*_bs batch, *_ts time) let an input be a channel slice of a wider
- * projection; outputs are packed.  lengths (int32 [B] or NULL): item b ends at row lengths[b] (clamped to 0 .. T); rows behind it are neither
- * read nor counted, their outputs and gradients are zero.  No atomics: results do not depend on timing.  Buffers that the caller sizes with a
+ * projection; outputs are packed.  lengths (int32 [B] or NULL): item b ends at row lengths[b] (clamped to 0 .. T); rows behind it count for
+ * nothing (whatever they hold), their outputs and gradients are zero.  No atomics: results do not depend on timing.  Buffers that the caller sizes with a
  * ga_*_sizes / ga_*_elems call need no initialisation. */
 
 /* Short causal depthwise convolution:  y[b][t][c] = act(bias[c] + sum_k w[c][k] x[b][t-(K-1)+k][c]), act GA_ACT_NONE or GA_ACT_SILU.
