@@ -46,8 +46,8 @@ Plan make_plan(int B, int T, int C, int N, int G) {
     q.nCb = q.cbg * G;
     q.tiles = (T + TS - 1) / TS;
     const long blocks = (long)B * q.nCb;
-    // Chunks for four blocks a CU, and for eight where a chunk is still long enough (16 tiles) not to notice its start: at 16 x 2250 x 1024 the
-    // forward kernel takes 247 us with two blocks a CU, 201 with four, 181 with eight; a 2250-row prompt of 8 blocks 37 us with four, 51 with eight.
+    // Chunks for four blocks a CU, and for eight where a chunk is still long enough (16 tiles) not to notice its start: the forward pass of
+    // 16 x 2250 x 1024 takes 287 us with eight, 295 with four, 311 with two; 12 x 375 x 512 39 us with four, 44 with eight.
     long want = (1024 + blocks - 1) / blocks;
     if (q.tiles / want >= 16) want = (2048 + blocks - 1) / blocks;
     if (want > MAX_CHUNKS) want = MAX_CHUNKS;
