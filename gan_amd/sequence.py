@@ -11,7 +11,9 @@ They take what a model around this package's convolutions, LSTM and GroupNorm la
 call in the same type), parameters, recurrent states and per-item conditions in float32.  All arithmetic, every sum and the states are float32;
 what is returned in bfloat16 is rounded once.  An activation may be a channel slice of a wider projection (unit stride along the channels);
 anything else that is not packed is copied.  Calls enqueue on the current stream of the tensors' device and keep nothing between calls, so they
-may be captured into graphs and run on several streams at once; results do not depend on timing (no atomics).  Gradients are of first order.
+may be captured into graphs and run on several streams at once; results do not depend on timing (no atomics).  Gradients are of first order; a
+backward pass is captured with torch.autograd.grad, or with leaves of which no eager graph is alive (a leaf's accumulation belongs to the
+stream that first used it).  delta = -inf (or the type's lowest value) is a step of zero: the row leaves the states as they are.
 Sizes and types are checked here (ValueError / TypeError); like every operator of this package these run on the GPU only.
 """
 from __future__ import annotations
