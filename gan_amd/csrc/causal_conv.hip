@@ -273,10 +273,10 @@ __global__ __launch_bounds__(256) void cconv_step_kernel(ga_causal_conv_step_par
 }
 
 int bad(int B, int T, int C, int K, int act, int dtype) {
-    if (B < 1 || T < 1 || C < 1 || K < 1 || K > GA_CCONV_MAX_TAPS || (act != GA_ACT_NONE && act != GA_ACT_SILU)) return GA_ERR_ARG;
+    if (B < 1 || T < 1 || T > 0x7fffffff - 256 || C < 1 || C > 0x7fffffff - 256 || K < 1 || K > GA_CCONV_MAX_TAPS || (act != GA_ACT_NONE && act != GA_ACT_SILU)) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Map m = make_map(B, T, C, 1);
-    if ((m.runs + m.ry - 1) / m.ry * m.pb > 0x7fffffffL || (long)T + 256 > 0x7fffffffL) return GA_ERR_ARG;
+    if ((m.runs + m.ry - 1) / m.ry * m.pb > 0x7fffffffL) return GA_ERR_ARG;
     return GA_OK;
 }
 

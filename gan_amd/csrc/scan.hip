@@ -946,10 +946,10 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, i
 }
 
 int bad_sizes(int B, int T, int C, int N, int G, int dtype) {
-    if (B < 1 || T < 1 || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
+    if (B < 1 || T < 1 || T > 0x7fffffff - TS || C < 1 || C > GA_SCAN_MAX_STRIDE || N < 1 || N > GA_SCAN_MAX_STATES || G < 1 || C % G) return GA_ERR_ARG;
     if (dtype != GA_DTYPE_F32 && dtype != GA_DTYPE_BF16) return GA_ERR_ARG;
     const Plan q = make_plan(B, T, C, N, G);
-    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 63) / 64 > 0x7fffffffUL || (long)T + TS > 0x7fffffffL)
+    if ((long)B * q.nCb * q.chunks > 0x7fffffffL || (long)B * G > 0x7fffffffL || ((size_t)B * N * C + 63) / 64 > 0x7fffffffUL)
         return GA_ERR_ARG;
     return GA_OK;
 }

@@ -712,3 +712,26 @@ def test_a_graph_that_saved_a_state_refuses_it_after_a_step():
         h2 = torch.zeros(2, 8, 3, device=DEV)
         S.selective_scan_step(x[:, 0], x[:, 1], -w[:, :3].abs(), w[:2, :3].contiguous(), w[2:4, :3].contiguous(), h2)
         assert bool((h2 != 0).any())
+
+
+@pytest.mark.parametrize("which", ["conv", "scan", "norm"])
+def test_backwards_twice_through_one_graph_and_from_a_broadcast_gradient(which):
+    """retain_graph: the same bits again (nothing that a backward pass reads is written by it); a gradient without memory of its own (of a sum)
+    is that of ones."""
+    g = gen(61)
+    if which == "conv":
+        leaves = [rnd(g, 2, 9, 12), rnd(g, 12, 3), rnd(g, 12)]
+        run = lambda x, w, b: S.causal_conv(x, w, b, L.ACT_SILU)  # noqa: E731
+    elif which == "scan":
+        leaves = [rnd(g, 2, 40, 12), rnd(g, 2, 40, 12) - 1, -rnd(g, 12, 5).abs(), rnd(g, 2, 40, 5), rnd(g, 2, 40, 5)]
+        run = S.selective_scan
+    else:
+        leaves = [rnd(g, 2, 9, 12), rnd(g, 2, 9, 12), rnd(g, 12)]
+        run = lambda x, b, w: S.block_norm(x, b, weight=w, post_norm=True)[1]  # noqa: E731
+    leaves = [t.requires_grad_() for t in leaves]
+    y = run(*leaves)
+    first = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+    again = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+    y.sum().backward()
+    for a, b, t in zip(first, again, leaves):
+        assert torch.equal(a, b) and torch.equal(a, t.grad)

@@ -214,3 +214,12 @@ def test_selective_scan_refuses_more_channels_than_its_offsets_reach():
     u = torch.zeros(1).expand(1, 1, Cn)
     with pytest.raises(ValueError, match="channels"):
         S.selective_scan(u, u, torch.zeros(1, 1).expand(Cn, 1), torch.zeros(1, 1, 1), torch.zeros(1, 1, 1))
+
+
+def test_c_entries_refuse_lengths_at_the_end_of_the_integers():
+    lib, s = L.lib(), L.ScanBuffers()
+    for T in (2 ** 31 - 1, 2 ** 31 - 16):
+        assert lib.ga_scan_sizes(1, T, 1, 1, 1, C.byref(s)) == 1
+        assert lib.ga_causal_conv_bwd_ws_elems(1, T, 1, 1) == 0
+    assert lib.ga_scan_sizes(2 ** 20, 2 ** 20, 2 ** 16, 1, 1, C.byref(s)) == 0  # 2^20 items of 1024 blocks: 2^30, a grid has up to 2^31 - 1
+    assert lib.ga_scan_sizes(2 ** 21, 2 ** 20, 2 ** 16, 1, 1, C.byref(s)) == 1  # 2^31
