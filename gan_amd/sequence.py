@@ -28,6 +28,9 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 
 Tensor = torch.Tensor
+_pack_conv, _pack_conv_bwd, _pack_conv_step = (L.packer(c) for c in (L.CausalConvParams, L.CausalConvBwdParams, L.CausalConvStepParams))
+_pack_scan, _pack_scan_bwd, _pack_scan_step = (L.packer(c) for c in (L.ScanParams, L.ScanBwdParams, L.ScanStepParams))
+_pack_norm, _pack_norm_bwd = L.packer(L.BlockNormParams), L.packer(L.BlockNormBwdParams)
 
 
 # ------------------------------------------------------------------------------------------------ checks and launching
@@ -50,12 +53,13 @@ def _lengths(t: Optional[Tensor], B: int) -> None:
 
 
 def _one_device(first: Tensor, *ts) -> None:
-    dev = first.device
+    index = first.get_device()
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             L.require_cuda(first, t)
-            raise RuntimeError(f"all tensors of a call must be on one device: got {dev} and {t.device}")
-    L.require_cuda(first)
+            raise RuntimeError(f"all tensors of a call must be on one device: got {first.device} and {t.device}")
+    if index < 0:
+        L.require_cuda(first)
 
 
 def _rows(t: Optional[Tensor]) -> Optional[Tensor]:
@@ -125,9 +129,9 @@ def _conv_fwd(x, weight, bias, act, state, lengths, want_last):
     K = weight.shape[1]
     y = x.new_empty(B, T, Cn)
     last = x.new_empty(B, K - 1, Cn) if want_last else None
-    p = L.CausalConvParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), y.data_ptr(),
-                           L.ptr(last) if K > 1 else 0, x.stride(0), x.stride(1), B, T, Cn, K, act)
-    _call("ga_causal_conv_fwd", x.device, C.byref(p), L.dt(x))
+    p = _pack_conv(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), y.data_ptr(),
+                   L.ptr(last) if K > 1 else 0, x.stride(0), x.stride(1), B, T, Cn, K, act)
+    _call("ga_causal_conv_fwd", x.device, p, L.dt(x))
     return y, last
 
 
@@ -154,10 +158,10 @@ class _CausalConv(torch.autograd.Function):
         dw = weight.new_empty(Cn, K)
         db = weight.new_empty(Cn) if bias is not None else None
         ws = weight.new_empty(L.lib().ga_causal_conv_bwd_ws_elems(B, T, Cn, K))
-        p = L.CausalConvBwdParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), dy.data_ptr(),
-                                  L.ptr(dlast), dx.data_ptr(), L.ptr(dstate) if K > 1 else 0, dw.data_ptr(), L.ptr(db), ws.data_ptr(),
-                                  x.stride(0), x.stride(1), B, T, Cn, K, ctx.act)
-        _call("ga_causal_conv_bwd", x.device, C.byref(p), L.dt(x))
+        p = _pack_conv_bwd(x.data_ptr(), weight.data_ptr(), L.ptr(bias), L.ptr(state) if K > 1 else 0, L.ptr(lengths), dy.data_ptr(),
+                           L.ptr(dlast), dx.data_ptr(), L.ptr(dstate) if K > 1 else 0, dw.data_ptr(), L.ptr(db), ws.data_ptr(),
+                           x.stride(0), x.stride(1), B, T, Cn, K, ctx.act)
+        _call("ga_causal_conv_bwd", x.device, p, L.dt(x))
         return dx, dw, db, dstate, None, None, None
 
 
@@ -219,9 +223,9 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     _one_device(x, weight, bias, state)
     x, weight, bias = _rows(x), _packed(weight), _packed(bias)
     y = x.new_empty(B, Cn)
-    p = L.CausalConvStepParams(x.data_ptr(), weight.data_ptr(), L.ptr(bias), state.data_ptr() if K > 1 else 0, y.data_ptr(), x.stride(0), bs, B, Cn,
-                               K, act)
-    _call("ga_causal_conv_step", x.device, C.byref(p), dt)
+    p = _pack_conv_step(x.data_ptr(), weight.data_ptr(), L.ptr(bias), state.data_ptr() if K > 1 else 0, y.data_ptr(), x.stride(0), bs, B, Cn,
+                        K, act)
+    _call("ga_causal_conv_step", x.device, p, dt)
     _moved_on(state)
     return y
 
@@ -248,10 +252,10 @@ def _scan_fwd(u, delta, A, Bm, Cm, D, z, delta_bias, softplus, state, lengths, w
     if n_ends:
         tmp = A.new_empty(n_ends + n_step) if want_hs else None
         ends = maps + 4 * n_maps if tmp is None else tmp.data_ptr()
-    p = L.ScanParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
-                     L.ptr(state), L.ptr(lengths), y.data_ptr(), L.ptr(last), maps, hs, ends, ends + 4 * n_ends, *u.stride()[:2], *delta.stride()[:2],
-                     *((0, 0) if z is None else z.stride()[:2]), *Bm.stride()[:2], *Cm.stride()[:2], B, T, Cn, N, G, softplus)
-    _call("ga_scan_fwd", u.device, C.byref(p), L.dt(u))
+    p = _pack_scan(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
+                   L.ptr(state), L.ptr(lengths), y.data_ptr(), L.ptr(last), maps, hs, ends, ends + 4 * n_ends, *u.stride()[:2], *delta.stride()[:2],
+                   *((0, 0) if z is None else z.stride()[:2]), *Bm.stride()[:2], *Cm.stride()[:2], B, T, Cn, N, G, softplus)
+    _call("ga_scan_fwd", u.device, p, L.dt(u))
     return y, last, keep
 
 
@@ -288,18 +292,18 @@ class _SelectiveScan(torch.autograd.Function):
         ends = ws.data_ptr()
         step, maps = ends + 4 * n_ends, keep.data_ptr()
         dmaps = step + 4 * n_step
-        p = L.ScanBwdParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), A.data_ptr(), L.ptr(D), L.ptr(delta_bias), L.ptr(lengths), dy.data_ptr(),
-                            L.ptr(dlast), maps, maps + 4 * n_maps, du.data_ptr(), ddelta.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr(),
-                            dA.data_ptr(), L.ptr(dD), L.ptr(dbias), L.ptr(dstate), ends, step, dmaps, dmaps + 4 * n_dmaps, *u.stride()[:2],
-                            *delta.stride()[:2], *((0, 0) if z is None else z.stride()[:2]), B, T, Cn, N, G, softplus)
-        _call("ga_scan_bwd", u.device, C.byref(p), L.dt(u))
+        p = _pack_scan_bwd(u.data_ptr(), delta.data_ptr(), L.ptr(z), A.data_ptr(), L.ptr(D), L.ptr(delta_bias), L.ptr(lengths), dy.data_ptr(),
+                           L.ptr(dlast), maps, maps + 4 * n_maps, du.data_ptr(), ddelta.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr(),
+                           dA.data_ptr(), L.ptr(dD), L.ptr(dbias), L.ptr(dstate), ends, step, dmaps, dmaps + 4 * n_dmaps, *u.stride()[:2],
+                           *delta.stride()[:2], *((0, 0) if z is None else z.stride()[:2]), B, T, Cn, N, G, softplus)
+        _call("ga_scan_bwd", u.device, p, L.dt(u))
         return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None
 
 
 def _scan_maps(name: str, t: Tensor, lead, Cn: int, dtype) -> Tensor:
     if t.dim() == len(lead) + 1:
         t = t.unsqueeze(-2)
-    if t.dim() != len(lead) + 2 or tuple(t.shape[:-2]) != tuple(lead):
+    if t.dim() != len(lead) + 2 or t.shape[:-2] != lead:
         raise ValueError(f"{name}: expected {tuple(lead)} + [G, N] (or + [N]), got {tuple(t.shape)}")
     G, N = t.shape[-2:]
     if not 1 <= N <= L.SCAN_MAX_STATES or G < 1 or Cn % G:
@@ -323,7 +327,9 @@ def _scan_checks(u, delta, A, Bm, Cm, D, z, delta_bias, state):
         raise ValueError(f"u: at most {L.SCAN_MAX_STRIDE} channels, got {Cn}")
     _act("delta", delta, u.shape, u.dtype)
     _act("z", z, u.shape, u.dtype)
-    Bm, Cm = _scan_maps("Bm", Bm, lead, Cn, u.dtype), _scan_maps("Cm", Cm, lead, Cn, u.dtype)
+    like = Bm.shape == Cm.shape and Bm.dtype == Cm.dtype
+    Bm = _scan_maps("Bm", Bm, lead, Cn, u.dtype)
+    Cm = (Cm if Cm.dim() == Bm.dim() else Cm.unsqueeze(-2)) if like else _scan_maps("Cm", Cm, lead, Cn, u.dtype)
     if Bm.shape != Cm.shape:
         raise ValueError(f"Bm and Cm differ in shape: {tuple(Bm.shape)} and {tuple(Cm.shape)}")
     N = Bm.shape[-1]
@@ -376,10 +382,10 @@ def selective_scan_step(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Ten
     _one_device(u, delta, A, Bm, Cm, D, z, delta_bias, state)
     u, delta, z, Bm, Cm, A, D, delta_bias = _rows(u), _rows(delta), _rows(z), _maps(Bm), _maps(Cm), _packed(A), _packed(D), _packed(delta_bias)
     y = u.new_empty(B, Cn)
-    p = L.ScanStepParams(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
-                         state.data_ptr(), y.data_ptr(), u.stride(0), delta.stride(0), 0 if z is None else z.stride(0), Bm.stride(0), Cm.stride(0), bs,
-                         B, Cn, N, G, int(softplus))
-    _call("ga_scan_step", u.device, C.byref(p), L.dt(u))
+    p = _pack_scan_step(u.data_ptr(), delta.data_ptr(), L.ptr(z), Bm.data_ptr(), Cm.data_ptr(), A.data_ptr(), L.ptr(D), L.ptr(delta_bias),
+                        state.data_ptr(), y.data_ptr(), u.stride(0), delta.stride(0), 0 if z is None else z.stride(0), Bm.stride(0), Cm.stride(0), bs,
+                        B, Cn, N, G, int(softplus))
+    _call("ga_scan_step", u.device, p, L.dt(u))
     _moved_on(state)
     return y
 
@@ -394,9 +400,9 @@ def _norm_fwd(x, branch, gate, w, b, wp, bp, scale, ab, post, layer, eps, dtype,
     y = x.new_empty((B, T, Cn), dtype=dtype)
     r = x.new_empty(B, T, Cn) if branch is not None else None
     stats = x.new_empty((B * T, 4), dtype=torch.float32) if want_stats else None
-    p = L.BlockNormParams(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab), L.ptr(r),
-                          y.data_ptr(), L.ptr(stats), B, T, Cn, int(post), int(layer), _gate_rows(gate), eps)
-    _call("ga_block_norm_fwd", x.device, C.byref(p), L.dt(x), L.dt(y))
+    p = _pack_norm(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab), L.ptr(r),
+                   y.data_ptr(), L.ptr(stats), B, T, Cn, int(post), int(layer), _gate_rows(gate), eps)
+    _call("ga_block_norm_fwd", x.device, p, L.dt(x), L.dt(y))
     return r, y, stats
 
 
@@ -423,10 +429,10 @@ class _BlockNorm(torch.autograd.Function):
         rows = _gate_rows(gate)
         by_item = ab is not None or (gate is not None and not rows)
         ws = stats.new_empty(L.lib().ga_block_norm_bwd_ws_elems(B, T, Cn, int(by_item)))
-        p = L.BlockNormBwdParams(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab),
-                                 stats.data_ptr(), L.ptr(dr), L.ptr(dy), dx.data_ptr(), L.ptr(dbranch), L.ptr(dgate), L.ptr(dw), L.ptr(db), L.ptr(dwp),
-                                 L.ptr(dbp), L.ptr(dscale), L.ptr(dab), ws.data_ptr(), B, T, Cn, int(post), int(layer), rows)
-        _call("ga_block_norm_bwd", x.device, C.byref(p), L.dt(x), L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F32)
+        p = _pack_norm_bwd(x.data_ptr(), L.ptr(branch), L.ptr(gate), L.ptr(w), L.ptr(b), L.ptr(wp), L.ptr(bp), L.ptr(scale), L.ptr(ab),
+                           stats.data_ptr(), L.ptr(dr), L.ptr(dy), dx.data_ptr(), L.ptr(dbranch), L.ptr(dgate), L.ptr(dw), L.ptr(db), L.ptr(dwp),
+                           L.ptr(dbp), L.ptr(dscale), L.ptr(dab), ws.data_ptr(), B, T, Cn, int(post), int(layer), rows)
+        _call("ga_block_norm_bwd", x.device, p, L.dt(x), L.DT_BF16 if dtype == torch.bfloat16 else L.DT_F32)
         return dx, dbranch, dgate, dw, db, dwp, dbp, dscale, dab, None, None, None, None
 
 
