@@ -11,9 +11,10 @@ They take what a model around this package's convolutions, LSTM and GroupNorm la
 call in the same type), parameters, recurrent states and per-item conditions in float32.  All arithmetic, every sum and the states are float32;
 what is returned in bfloat16 is rounded once.  An activation may be a channel slice of a wider projection (unit stride along the channels);
 anything else that is not packed is copied.  Calls enqueue on the current stream of the tensors' device and keep nothing between calls, so they
-may be captured into graphs and run on several streams at once; results do not depend on timing (no atomics).  Gradients are of first order; a
-backward pass is captured with torch.autograd.grad, or with leaves of which no eager graph is alive (a leaf's accumulation belongs to the
-stream that first used it).  delta = -inf (or the type's lowest value) is a step of zero: the row leaves the states as they are.
+may be captured into graphs and run on several streams at once; results do not depend on timing (no atomics).  Gradients are of first order and in
+reverse mode (a tensor with a forward-mode tangent is refused, NotImplementedError); a backward pass is captured with torch.autograd.grad, or
+with leaves of which no eager graph is alive (a leaf's accumulation belongs to the stream that first used it).  delta = -inf (or the type's
+lowest value) is a step of zero: the row leaves the states as they are.
 Sizes and types are checked here (ValueError / TypeError); like every operator of this package these run on the GPU only.
 """
 from __future__ import annotations
@@ -23,6 +24,7 @@ from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -96,6 +98,14 @@ def _wants_grad(*ts) -> bool:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _no_tangents(name: str, *ts) -> None:
+    """A dual tensor asks for no gradient: past this check its tangent would be dropped without a word."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _no_grad_step(name: str, whole: str, *ts) -> None:
@@ -197,6 +207,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: i
     _conv_act(act)
     _act("state", state, (B, weight.shape[1] - 1, Cn), x.dtype)
     _lengths(lengths, B)
+    _no_tangents("causal_conv", x, weight, bias, state)
     _one_device(x, weight, bias, state, lengths)
     x, weight, bias, state, lengths = _rows(x), _packed(weight), _packed(bias), _packed(state), _packed(lengths)
     if _wants_grad(x, weight, bias, state):
@@ -219,6 +230,7 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     _conv_act(act)
     _act("state", state, (B, K - 1, Cn), x.dtype)
     bs = _state_rows("state", state, (K - 1) * Cn) if K > 1 else 0
+    _no_tangents("causal_conv_step", x, weight, bias, state)
     _no_grad_step("causal_conv_step", "causal_conv", x, weight, bias, state)
     _one_device(x, weight, bias, state)
     x, weight, bias = _rows(x), _packed(weight), _packed(bias)
@@ -356,6 +368,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Tensor, 
         raise ValueError(f"u: expected a non-empty [B, T, C], got {tuple(u.shape)}")
     Bm, Cm = _scan_checks(u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _lengths(lengths, u.shape[0])
+    _no_tangents("selective_scan", u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _one_device(u, delta, A, Bm, Cm, D, z, delta_bias, state, lengths)
     u, delta, z, Bm, Cm = _scan_rows(u), _scan_rows(delta), _scan_rows(z), _maps(Bm), _maps(Cm)
     A, D, delta_bias, state, lengths = _packed(A), _packed(D), _packed(delta_bias), _packed(state), _packed(lengths)
@@ -378,6 +391,7 @@ def selective_scan_step(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Ten
     B, Cn = u.shape
     G, N = Bm.shape[1:]
     bs = _state_rows("state", state, Cn * N)
+    _no_tangents("selective_scan_step", u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _no_grad_step("selective_scan_step", "selective_scan", u, delta, A, Bm, Cm, D, z, delta_bias, state)
     _one_device(u, delta, A, Bm, Cm, D, z, delta_bias, state)
     u, delta, z, Bm, Cm, A, D, delta_bias = _rows(u), _rows(delta), _rows(z), _maps(Bm), _maps(Cm), _packed(A), _packed(D), _packed(delta_bias)
@@ -485,6 +499,7 @@ def block_norm(x: Tensor, branch: Optional[Tensor] = None, *, weight: Optional[T
             _act("gate", gate, (B, T, Cn), dtype)
     _vec("ab", ab, B, 2 * Cn)
     ts = (branch, gate, weight, bias, post_weight, post_bias, scale, ab)
+    _no_tangents("block_norm", x, *ts)
     _one_device(x, *ts)
     ts = tuple(_packed(t) for t in ts)
     xc = x.contiguous()

@@ -1,0 +1,35 @@
+"""CPU: calls of the sequence operators that have to be refused by name, before anything touches a GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from gan_amd import sequence as S
+
+ARGS = {
+    "causal_conv": lambda: dict(x=torch.randn(2, 5, 8), weight=torch.randn(8, 4), bias=torch.randn(8), state=torch.randn(2, 3, 8)),
+    "causal_conv_step": lambda: dict(x=torch.randn(2, 8), state=torch.randn(2, 3, 8), weight=torch.randn(8, 4), bias=torch.randn(8)),
+    "selective_scan": lambda: dict(u=torch.randn(2, 5, 8), delta=torch.randn(2, 5, 8), A=-torch.rand(8, 6), Bm=torch.randn(2, 5, 6), Cm=torch.randn(2, 5, 6),
+                                   D=torch.randn(8), z=torch.randn(2, 5, 8), delta_bias=torch.randn(8), state=torch.randn(2, 8, 6)),
+    "selective_scan_step": lambda: dict(u=torch.randn(2, 8), delta=torch.randn(2, 8), A=-torch.rand(8, 6), Bm=torch.randn(2, 6), Cm=torch.randn(2, 6),
+                                        state=torch.randn(2, 8, 6), D=torch.randn(8), z=torch.randn(2, 8), delta_bias=torch.randn(8)),
+    "block_norm": lambda: dict(x=torch.randn(2, 5, 8), branch=torch.randn(2, 5, 8), weight=torch.randn(8), bias=torch.randn(8), post_norm=True,
+                               post_weight=torch.randn(8), post_bias=torch.randn(8), gate=torch.randn(2, 5, 8), scale=torch.randn(8), ab=torch.randn(2, 16)),
+}
+TENSORS = [(op, k) for op, make in ARGS.items() for k, v in make().items() if torch.is_tensor(v)]
+
+
+@pytest.mark.parametrize("grad", [True, False], ids=["", "no_grad"])
+@pytest.mark.parametrize("op, which", TENSORS)
+def test_forward_mode_derivatives_are_refused(op, which, grad):
+    """A dual tensor does not ask for gradients; its tangent would be lost in silence."""
+    a = ARGS[op]()
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        a[which] = fwd.make_dual(a[which], torch.randn_like(a[which]))
+        with pytest.raises(NotImplementedError, match=f"{op}.*forward-mode"):
+            getattr(S, op)(**a)
+
+
+@pytest.mark.parametrize("op", ARGS)
+def test_tensors_without_a_tangent_pass_inside_a_dual_level(op):
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="GPU only"):
+        getattr(S, op)(**ARGS[op]())
