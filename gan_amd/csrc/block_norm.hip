@@ -87,7 +87,11 @@ __device__ __forceinline__ void convert(float (&o)[P][V], const Pack<T, V> (&r)[
     BN_EACH o[i][e] = (float)r[i].v[e];
 }
 
-// (mean, 1 / sqrt(variance or mean square + eps)) of R rows; the variance about the mean, in a second sum
+// (mean, 1 / sqrt(variance or mean square + eps)) of R rows; the variance about the mean, in a second sum.  The squares are of v 2^-8 and their mean
+// is multiplied by 2^16 again: 4096 squares of 1e18 add up to 4e39, beyond float32, where their mean is not.  (Both factors are exact, and the first
+// comes with the subtraction: the same bits and the same instructions as without.  Squares that get below float32's normal numbers that way, 8e-34, are
+// nothing beside an eps of 1e-30 to 24 bits, denormal as they are.)
+constexpr float SQ_DOWN = 1.f / 256.f, SQ_UP = 65536.f;
 template <int G, int P, int V, int R>
 __device__ __forceinline__ void row_stats(const float (&v)[R][P][V], float (&mean)[R], float (&rstd)[R], const bool (&in)[P], float inv, bool layer,
                                           float eps, float (*red)[8][16], int& slot) {
@@ -104,12 +108,12 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][P][V], float (&mea
     BN_ROWS {
         s[j] = 0.f;
         BN_EACH {
-            const float t = in[i] ? v[j][i][e] - mean[j] : 0.f;
+            const float t = in[i] ? fmaf(v[j][i][e], SQ_DOWN, -SQ_DOWN * mean[j]) : 0.f;
             s[j] = fmaf(t, t, s[j]);
         }
     }
     row_sums<G, R>(s, red, slot);
-    BN_ROWS rstd[j] = 1.f / sqrtf(fmaf(s[j], inv, eps));
+    BN_ROWS rstd[j] = 1.f / sqrtf(fmaf(s[j], inv * SQ_UP, eps));
 }
 
 // G threads a row, P pieces of V columns a thread, R rows at a time: their loads are in flight together and their sums share the exchanges.

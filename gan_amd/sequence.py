@@ -461,7 +461,7 @@ def block_norm(x: Tensor, branch: Optional[Tensor] = None, *, weight: Optional[T
         y = (norm(r) * weight + bias) * (1 + a) + s       ab = (a | s)
 
     norm(v) = v / sqrt(mean(v^2) + eps) (kind "rms") or (v - mean) / sqrt(var + eps) (kind "layer") over the C <= 4096 channels (|v| up to
-    1e18: the squares are float32).
+    1e18: mean squares are float32).
     x [B, T, C] is the residual stream, float32 or the branch's type, and r has x's type; branch and y are in the activations' type (`dtype` names
     it when there is no branch; x's by default).  weight, bias, post_weight, post_bias, scale: float32 [C] or None (1 or 0).  gate: float32 [B, C]
     (one vector an item) or [B, T, C] in the branch's type.  ab: float32 [B, 2C], as GnFilmAct takes it.  Without a branch (the first block) r is x.
