@@ -235,6 +235,14 @@ __device__ __forceinline__ void get_sum2(float (&x)[4], float (&y)[4], float2 (*
         }
 }
 
+// 2^s c + end for any s.  The steps of a chunk may grow a state (A > 0, or negative steps) by more than float32 holds although the state itself, small or
+// exactly zero, stays inside: powers of two above 2^126 go into c's exponent, where zero stays zero.  (c < 2^128 is at least 2^-149: beyond s = 277 what
+// is not zero is infinite.  Up to s = 126 the bits are those of exp2(s) c + end; a NaN passes on.)
+__device__ __forceinline__ float grown(float s, float c, float end) {
+    const float t = s > 400.f ? 400.f : s, over = fmaxf(ceilf(t) - 126.f, 0.f);
+    return fmaf(__builtin_amdgcn_exp2f(t - over), __builtin_ldexpf(c, (int)over), end);
+}
+
 // What comes into each chunk, from what each one leaves behind by itself, in place: carry' = exp(A sum of steps) carry + end, over the chunks
 // in order (forward) or against it (backward: dir < 0), from `first` [B][C][N] (or zero).  A wave takes 64 states and one of SEGS runs of up to U
 // chunks, all their loads in flight at once (few threads, a long way to memory); with more runs than one each is first walked from zero, and the
@@ -266,20 +274,20 @@ __global__ __launch_bounds__(SEGS > 1 ? SEGS * 64 : 256) void scan_carry_kernel(
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (k0 + u < k1) {
-                e = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), e, end[u]);
+                e = grown(sum[u] * A2, e, end[u]);
                 total += sum[u];
             }
         se[seg][lane] = e;
         st[seg][lane] = total;
         __syncthreads();
-        for (int j = 0; j < seg; ++j) c = fmaf(__builtin_amdgcn_exp2f(st[j][lane] * A2), c, se[j][lane]);
+        for (int j = 0; j < seg; ++j) c = grown(st[j][lane] * A2, c, se[j][lane]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (k0 + u < k1 && id < all) {
             const int chunk = dir < 0 ? q.chunks - 1 - (k0 + u) : k0 + u;
             ep[(size_t)chunk * q.NP * C] = c;
-            c = fmaf(__builtin_amdgcn_exp2f(sum[u] * A2), c, end[u]);  // (what the last chunk leaves is written by no block, and used here by nobody)
+            c = grown(sum[u] * A2, c, end[u]);  // (what the last chunk leaves is written by no block, and used here by nobody)
         }
 }
 

@@ -360,9 +360,10 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Tensor, 
         h[b, t, c, n] = exp(step * A[c, n]) * h[b, t-1, c, n] + step * u[b, t, c] * Bm[b, t, g, n]
         y[b, t, c]    = (sum_n Cm[b, t, g, n] * h[b, t, c, n] + D[c] * u[b, t, c]) * silu(z[b, t, c])
 
-    u, delta, z [B, T, C]; Bm, Cm [B, T, G, N] (or [B, T, N]), channel c reads group g = c // (C / G), N <= 64; A [C, N] (negative for a decay),
-    D, delta_bias [C], state [B, C, N] (the states before row 0, zero without it): float32.  `lengths` as in causal_conv: rows behind an
-    item's end leave its state alone, give y = 0 and get no gradient.  With `return_state` also the states at each item's end, float32 [B, C, N].
+    u, delta, z [B, T, C]; Bm, Cm [B, T, G, N] (or [B, T, N]), channel c reads group g = c // (C / G), N <= 64; A [C, N] (negative for a decay; a
+    single row's factor exp(step * A) has to be inside float32, the product over many rows need not), D, delta_bias [C], state [B, C, N] (the
+    states before row 0, zero without it): float32.  `lengths` as in causal_conv: rows behind an item's end leave its state alone, give y = 0 and
+    get no gradient.  With `return_state` also the states at each item's end, float32 [B, C, N].
     Differentiable in every tensor but `lengths`; the backward pass keeps the state at every 16th row (C * N / 16 floats a row)."""
     if u.dim() != 3 or 0 in u.shape:
         raise ValueError(f"u: expected a non-empty [B, T, C], got {tuple(u.shape)}")
