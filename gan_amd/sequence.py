@@ -228,6 +228,8 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     K = weight.shape[1]
     _vec("bias", bias, Cn)
     _conv_act(act)
+    if state is None:
+        raise ValueError("state: a [B, K - 1, C] tensor expected")
     _act("state", state, (B, K - 1, Cn), x.dtype)
     bs = _state_rows("state", state, (K - 1) * Cn) if K > 1 else 0
     _no_tangents("causal_conv_step", x, weight, bias, state)

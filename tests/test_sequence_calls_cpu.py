@@ -33,3 +33,11 @@ def test_forward_mode_derivatives_are_refused(op, which, grad):
 def test_tensors_without_a_tangent_pass_inside_a_dual_level(op):
     with fwd.dual_level(), pytest.raises(RuntimeError, match="GPU only"):
         getattr(S, op)(**ARGS[op]())
+
+
+def test_causal_conv_step_without_a_state():
+    a = ARGS["causal_conv_step"]()
+    with pytest.raises(ValueError, match="state"):
+        S.causal_conv_step(**dict(a, state=None))
+    with pytest.raises(ValueError, match="state"):
+        S.causal_conv_step(a["x"], None, a["weight"][:, :1])
