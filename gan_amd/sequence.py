@@ -30,6 +30,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 
 Tensor = torch.Tensor
+FLOAT_MAX = torch.finfo(torch.float32).max
 _pack_conv, _pack_conv_bwd, _pack_conv_step = (L.packer(c) for c in (L.CausalConvParams, L.CausalConvBwdParams, L.CausalConvStepParams))
 _pack_scan, _pack_scan_bwd, _pack_scan_step = (L.packer(c) for c in (L.ScanParams, L.ScanBwdParams, L.ScanStepParams))
 _pack_norm, _pack_norm_bwd = L.packer(L.BlockNormParams), L.packer(L.BlockNormBwdParams)
@@ -477,7 +478,7 @@ def block_norm(x: Tensor, branch: Optional[Tensor] = None, *, weight: Optional[T
     L.dt(x)
     if kind not in ("rms", "layer"):
         raise ValueError(f"kind: 'rms' or 'layer' expected, got {kind!r}")
-    if not 1e-30 <= eps < float("inf"):
+    if not 1e-30 <= eps <= FLOAT_MAX:
         raise ValueError(f"eps: a positive number that float32 holds expected (1e-30 or more), got {eps}")
     if branch is None:
         if post_norm or post_weight is not None or post_bias is not None or gate is not None or scale is not None:

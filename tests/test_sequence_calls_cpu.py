@@ -41,3 +41,15 @@ def test_causal_conv_step_without_a_state():
         S.causal_conv_step(**dict(a, state=None))
     with pytest.raises(ValueError, match="state"):
         S.causal_conv_step(a["x"], None, a["weight"][:, :1])
+
+
+@pytest.mark.parametrize("eps", [1e39, 3.5e38, torch.finfo(torch.float32).max * 1.0000001, 1e300])
+def test_block_norm_refuses_an_eps_beyond_float32(eps):
+    with pytest.raises(ValueError, match="eps"):
+        S.block_norm(torch.randn(2, 5, 8), eps=eps)
+
+
+def test_block_norm_takes_the_largest_eps():
+    assert len(S._pack_norm(*[0] * 18, torch.finfo(torch.float32).max)) > 0
+    with pytest.raises(RuntimeError, match="GPU only"):
+        S.block_norm(torch.randn(2, 5, 8), eps=torch.finfo(torch.float32).max)
