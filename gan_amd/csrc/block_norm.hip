@@ -495,7 +495,7 @@ int ga_block_norm_bwd(const ga_block_norm_bwd_params* hp, int xdtype, int dtype,
     const size_t xb = xdtype == GA_DTYPE_BF16 ? 8 : 16, ob = dtype == GA_DTYPE_BF16 ? 8 : 16;
     const bool vec = p.C % 4 == 0 && aligned(p.x, xb) && aligned(p.dr, xb) && aligned(p.dx, xb) && aligned(p.branch, ob) && aligned(p.dy, ob) &&
                      aligned(p.dbranch, ob) && (!p.gate_rows || (aligned(p.gate, ob) && aligned(p.dgate, ob)));
-    if (!aligned(p.stats, 16)) return GA_ERR_ALIGN;
+    if (!aligned(p.stats, 16) || !aligned(p.ws, 16)) return GA_ERR_ALIGN;
     return by_type(p, xdtype, dtype, vec, Bwd{s});
 }
 

@@ -616,8 +616,8 @@ typedef struct ga_block_norm_params {
     float eps;
 } ga_block_norm_params;
 int ga_block_norm_fwd(const ga_block_norm_params* h_params, int xdtype, int dtype, ga_stream_t stream);
-/* dr (xdtype) and / or dy (dtype) -> dx (xdtype), dbranch, dgate (like gate), dab, dw, db, dwp, dbp, dscale (fp32, each may be NULL); ws: fp32,
- * ga_block_norm_bwd_ws_elems(..., by_item = there is an ab or a gate per item) */
+/* dr (xdtype) and / or dy (dtype) -> dx (xdtype), dbranch, dgate (like gate), dab, dw, db, dwp, dbp, dscale (fp32, each may be NULL); ws: fp32, 16-byte
+ * aligned like stats, ga_block_norm_bwd_ws_elems(..., by_item = there is an ab or a gate per item) */
 typedef struct ga_block_norm_bwd_params {
     const void* x; const void* branch; const void* gate;
     const float* w; const float* b; const float* wp; const float* bp; const float* scale; const float* ab;

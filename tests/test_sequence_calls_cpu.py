@@ -53,3 +53,15 @@ def test_block_norm_takes_the_largest_eps():
     assert len(S._pack_norm(*[0] * 18, torch.finfo(torch.float32).max)) > 0
     with pytest.raises(RuntimeError, match="GPU only"):
         S.block_norm(torch.randn(2, 5, 8), eps=torch.finfo(torch.float32).max)
+
+
+def test_c_entry_refuses_a_misaligned_workspace():
+    """The block norms' column sums leave in 16-byte pieces."""
+    import ctypes as C
+
+    from gan_amd import _lib as L
+    one = 1 << 20  # a non-null address that no refusal reads
+    p = L.BlockNormBwdParams(x=one, stats=one, dy=one, dx=one, B=1, T=1, C=8)
+    for off in (4, 8, 12):
+        p.ws = one + off
+        assert L.lib().ga_block_norm_bwd(C.byref(p), 0, 0, None) == 3
