@@ -403,6 +403,7 @@ struct Fwd {
         constexpr int threads = G == 64 ? 256 : G;
         static const int most = resident_blocks(bnorm_fwd_kernel<TX, TO, G, P, V, R>, threads);
         const Grid g = make_grid(p.B, p.T, p.ab || (p.gate && !p.gate_rows), (G == 64 ? 4 : 1) * R, most);
+        if (!sq_launch_fits((size_t)g.items * g.parts, threads)) return GA_ERR_ARG;
         bnorm_fwd_kernel<TX, TO, G, P, V, R><<<(unsigned)(g.items * g.parts), threads, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();
         return GA_OK;
@@ -416,6 +417,7 @@ struct Bwd {
         constexpr int threads = G == 64 ? 256 : G;
         static const int most = resident_blocks(bnorm_bwd_kernel<TX, TO, G, P, V, R>, threads);
         const Grid g = make_grid(p.B, p.T, by_item, (G == 64 ? 4 : 1) * R, most);
+        if (!sq_launch_fits((size_t)g.items * g.parts, threads)) return GA_ERR_ARG;
         const int blocks = g.items * g.parts;
         bnorm_bwd_kernel<TX, TO, G, P, V, R><<<(unsigned)blocks, threads, 0, s>>>(p, g.rows_per_item, g.parts);
         GA_CHECK_LAUNCH();

@@ -289,7 +289,9 @@ int parts_of(const Map& m) {
 template <typename T, int V, int K>
 int fwd(const ga_causal_conv_params& p, hipStream_t s) {
     const Map m = make_map(p.B, p.T, p.C, V);
-    cconv_fwd_kernel<T, V, K><<<(unsigned)((m.runs + m.ry - 1) / m.ry * m.pb), 256, 0, s>>>(p, m);
+    const size_t blocks = (size_t)((m.runs + m.ry - 1) / m.ry) * m.pb;
+    if (!sq_launch_fits(blocks, 256)) return GA_ERR_ARG;
+    cconv_fwd_kernel<T, V, K><<<(unsigned)blocks, 256, 0, s>>>(p, m);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
@@ -297,9 +299,11 @@ template <typename T, int V, int K>
 int bwd(const ga_causal_conv_bwd_params& p, hipStream_t s) {
     const Map m = make_map(p.B, p.T, p.C, V);
     const int parts = parts_of(m);
+    const size_t sums = ((size_t)(K + 1) * p.C + 31) / 32;
+    if (!sq_launch_fits((size_t)parts * m.pb, 256) || !sq_launch_fits(sums, 1024)) return GA_ERR_ARG;
     cconv_bwd_kernel<T, V, K><<<(unsigned)(parts * m.pb), 256, 0, s>>>(p, m, parts);
     GA_CHECK_LAUNCH();
-    cconv_dw_kernel<<<(unsigned)(((long)(K + 1) * p.C + 31) / 32), 1024, 0, s>>>(p.ws, parts, K, p.C, p.dw, p.dbias);
+    cconv_dw_kernel<<<(unsigned)sums, 1024, 0, s>>>(p.ws, parts, K, p.C, p.dw, p.dbias);
     GA_CHECK_LAUNCH();
     return GA_OK;
 }
@@ -370,7 +374,7 @@ int ga_causal_conv_step(const ga_causal_conv_step_params* hp, int dtype, hipStre
     if (rc) return rc;
     if (!p.x || !p.w || !p.y || (p.K > 1 && !p.state)) return GA_ERR_ARG;
     const size_t blocks = ((size_t)p.B * p.C + 255) / 256;
-    if (blocks > 0x7fffffffUL) return GA_ERR_ARG;
+    if (!sq_launch_fits(blocks, 256)) return GA_ERR_ARG;
     if (dtype == GA_DTYPE_BF16) cconv_step_kernel<bf16_t><<<(unsigned)blocks, 256, 0, s>>>(p);
     else cconv_step_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(p);
     GA_CHECK_LAUNCH();

@@ -974,7 +974,7 @@ int grid_for(size_t n) {
 }
 
 int launch_carry(const float* A, const float* first, float* ends, const float* ends_step, const Plan& q, int B, int C, int N, int dir, hipStream_t s) {
-    const size_t states = (size_t)B * N * C;
+    const size_t states = (size_t)B * N * C;  // (2^23 at the most: sequences are cut where there are fewer than 2048 blocks of 64 channels)
     static_assert(MAX_CHUNKS <= 16 * 16, "runs of the carry kernel");
     // (8 chunks at 16 x 2250 x 1024: 5.6 us, 8.3 with loads for 32; 32 chunks at 4 x 2250 x 512: the whole forward pass 62 us, 67 with 16 runs)
     if (q.chunks <= 8) scan_carry_kernel<1, 8><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
@@ -1072,6 +1072,7 @@ int ga_scan_fwd(const ga_scan_params* hp, int dtype, hipStream_t s) {
     if (rc) return rc;
     Args a{p, make_plan(p.B, p.T, p.C, p.N, p.G), 0};
     if (!p.u || !p.delta || !p.A || !p.Bm || !p.Cm || !p.y || !p.maps || (a.q.chunks > 1 && (!p.ends || !p.ends_step))) return GA_ERR_ARG;
+    if (!sq_launch_fits((size_t)p.B * a.q.nCb * a.q.chunks, 256)) return GA_ERR_ARG;
     if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
     const size_t el = dtype == GA_DTYPE_BF16 ? 2 : 4;
@@ -1089,6 +1090,7 @@ int ga_scan_bwd(const ga_scan_bwd_params* hp, int dtype, hipStream_t s) {
     if (!p.u || !p.delta || !p.A || !p.dy || !p.maps || !p.hs || !p.du || !p.ddelta || !p.dA || !p.dBm || !p.dCm || !p.dmaps || !p.dparams ||
         (!p.z) != (!p.dz) || (a.q.chunks > 1 && (!p.ends || !p.ends_step)))
         return GA_ERR_ARG;
+    if (!sq_launch_fits((size_t)p.B * a.q.nCb * a.q.chunks, 256) || !sq_launch_fits(((size_t)(a.q.NP + 2) * p.C + 31) / 32, 1024)) return GA_ERR_ARG;
     if (bad_strides(p.u_ts, p.delta_ts, p.z_ts)) return GA_ERR_ARG;
     if ((uintptr_t)p.maps & 15) return GA_ERR_ALIGN;
     const size_t el = dtype == GA_DTYPE_BF16 ? 2 : 4;
@@ -1106,7 +1108,7 @@ int ga_scan_step(const ga_scan_step_params* hp, int dtype, hipStream_t s) {
     int shift = 0;
     while ((4 << shift) < p.N) ++shift;
     const size_t nb = ((size_t)p.C + (256 >> shift) - 1) / (256 >> shift), blocks = nb * p.B;
-    if (blocks > 0x7fffffffUL) return GA_ERR_ARG;
+    if (!sq_launch_fits(blocks, 256)) return GA_ERR_ARG;
     const bool vec = p.N % 4 == 0 && p.state_bs % 4 == 0 && p.b_bs % 4 == 0 && p.c_bs % 4 == 0 && !(((uintptr_t)p.state | (uintptr_t)p.A) & 15) &&
                      !(((uintptr_t)p.Bm | (uintptr_t)p.Cm) & (dtype == GA_DTYPE_BF16 ? 7 : 15));
     if (dtype == GA_DTYPE_BF16) {

@@ -42,6 +42,9 @@ __device__ __forceinline__ int sq_len(const int* lengths, int b, int T) {
     return n < 0 ? 0 : n > T ? T : n;
 }
 
+// A launch has at most 2^32 - 1 work-items along an axis.
+inline bool sq_launch_fits(size_t blocks, size_t threads) { return blocks <= 0xffffffffUL / threads; }
+
 // Sums over the 64 lanes of many values at once: each step sends one half of the values each way across a lane bit, so that the work halves
 // with it (V values cost 2V - 2 exchanges and adds and not 6V).  permlane swaps for the upper two lane bits, DPP for the others.
 template <int CTRL>

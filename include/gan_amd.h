@@ -523,7 +523,8 @@ int ga_lstm_bwd(const ga_lstm_bwd_params* h_params, ga_stream_t stream);
  * No reference call site: they extend the operator set.  Element strides (*_bs batch, *_ts time) let an input be a channel slice of a wider
  * projection; outputs are packed.  lengths (int32 [B] or NULL): item b ends at row lengths[b] (clamped to 0 .. T); rows behind it count for
  * nothing (whatever they hold), their outputs and gradients are zero.  No atomics: results do not depend on timing.  Buffers that the caller sizes with a
- * ga_*_sizes / ga_*_elems call need no initialisation. */
+ * ga_*_sizes / ga_*_elems call need no initialisation.  Sizes whose launch would have 2^32 work-items or more (2^24 blocks of 256: items, 64-channel
+ * blocks and chunks multiplied) are refused before anything is enqueued. */
 
 /* Short causal depthwise convolution:  y[b][t][c] = act(bias[c] + sum_k w[c][k] x[b][t-(K-1)+k][c]), act GA_ACT_NONE or GA_ACT_SILU.
  * Rows before 0 come from state [B][K-1][C] (NULL: zero); last [B][K-1][C] (may be NULL) receives the K-1 rows that end the sequence. */

@@ -65,3 +65,30 @@ def test_c_entry_refuses_a_misaligned_workspace():
     for off in (4, 8, 12):
         p.ws = one + off
         assert L.lib().ga_block_norm_bwd(C.byref(p), 0, 0, None) == 3
+
+
+@pytest.mark.parametrize("entry, cls, sizes, absent", [
+    ("ga_causal_conv_fwd", "CausalConvParams", dict(B=1 << 30, T=1, C=64, K=2), ()),
+    ("ga_causal_conv_bwd", "CausalConvBwdParams", dict(B=1, T=1, C=1 << 30, K=2), ()),
+    ("ga_causal_conv_step", "CausalConvStepParams", dict(B=1 << 16, C=1 << 16, K=2), ()),
+    ("ga_scan_fwd", "ScanParams", dict(B=1 << 24, T=1, C=1, N=1, G=1), ()),
+    ("ga_scan_bwd", "ScanBwdParams", dict(B=1 << 24, T=1, C=1, N=1, G=1), ()),
+    ("ga_scan_bwd", "ScanBwdParams", dict(B=1, T=1, C=(1 << 22) - 1, N=64, G=1), ()),
+    ("ga_scan_step", "ScanStepParams", dict(B=1 << 24, C=1, N=1, G=1), ()),
+    ("ga_block_norm_fwd", "BlockNormParams", dict(B=1 << 24, T=1, C=8, eps=1e-5), ("branch", "gate")),
+    ("ga_block_norm_bwd", "BlockNormBwdParams", dict(B=1 << 24, T=1, C=8), ("branch", "gate")),
+    ("ga_block_norm_bwd", "BlockNormBwdParams", dict(B=1 << 24, T=1, C=8), ("ab",)),
+])
+def test_c_entries_refuse_more_work_items_than_a_launch_holds(entry, cls, sizes, absent):
+    """A launch has at most 2^32 - 1 work-items along an axis: 2^24 - 1 blocks of 256.  Every buffer is there, nothing but the sizes is wrong."""
+    import ctypes as C
+
+    from gan_amd import _lib as L
+    p = getattr(L, cls)()
+    for name, kind in p._fields_:
+        if kind is C.c_void_p and name not in absent:
+            setattr(p, name, 1 << 20)  # a non-null address that no refusal reads
+    for k, v in sizes.items():
+        setattr(p, k, v)
+    args = (0, 0, None) if "norm" in entry else (0, None)
+    assert getattr(L.lib(), entry)(C.byref(p), *args) == 1
