@@ -29,10 +29,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     headers = [CSRC / "common.h", CSRC / "swin_common.h", CSRC / "seq_common.h", HERE.parent / "include" / "gan_amd.h"]
     objdir = CSRC / "build"
     objdir.mkdir(exist_ok=True)
+    command = objdir / "command.txt"  # what the objects were compiled with: other flags or another compiler compile them all again
+    same = command.exists() and command.read_text() == repr([hipcc, *FLAGS])
     jobs = []
     for src in SOURCES:
         obj = objdir / (src + ".o")
-        if force or _stale(obj, [CSRC / src] + headers):
+        if force or not same or _stale(obj, [CSRC / src] + headers):
             jobs.append([hipcc, *FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
 
     def run(cmd):
@@ -44,10 +46,13 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if verbose and r.stderr.strip():
             print(r.stderr)
 
+    if not same:
+        command.unlink(missing_ok=True)  # (until all of them are)
     with ThreadPoolExecutor(max_workers=min(6, max(1, len(jobs)))) as ex:
         list(ex.map(run, jobs))
+    command.write_text(repr([hipcc, *FLAGS]))
     objs = [str(objdir / (s + ".o")) for s in SOURCES]
-    if force or jobs or not LIB.exists():
+    if force or jobs or _stale(LIB, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(LIB), *objs])
     return LIB
 
