@@ -7,8 +7,9 @@
 // A row is held in the registers of 64 lanes (one wave) or of a whole block.  Column sums (the parameters' gradients) stay in registers over a
 // block's rows and leave as one row of partial sums per block, added up in a fixed order: results do not depend on timing.
 //
-// Measured at 16 x 2250 x 1024, residual float32, the rest bf16, a gate per row: forward 105 us (516 MB: 4.9 TB/s, what a large copy reaches),
-// backward 159 us (811 MB: 5.1 TB/s) and 10 us for the parameter sums.  64 x 375 x 512 bf16: 22 and 39 us; one row of 64 items: 5 us.
+// Measured at 16 x 2250 x 1024, residual float32, the rest bf16, a gate per row: forward 106 us (516 MB: 4.9 TB/s, what a large copy reaches),
+// backward 159 us (811 MB: 5.1 TB/s) and 10 us for the parameter sums; all float32 148 us (737 MB: 5.0 TB/s) and 251 us with the sums (1180 MB:
+// 4.7 TB/s).  64 x 375 x 512 bf16: 22 and 38 us, float32 34 and 61; one row of 64 items: 5 us.
 #include "seq_common.h"
 
 namespace {
@@ -369,7 +370,8 @@ struct Grid {
     long rows_per_item;
 };
 // Without vectors of their own the items are one long item.  As many blocks as fit the card at once (`most`: more leave a last, partly filled
-// round, measured 170 us at three blocks a CU and 227 at four where three fit), and no more than the same number of turns over the rows needs.
+// round: 64 x 375 x 512 bf16 takes 21.7 + 38.4 us, 24.8 + 44.7 with four blocks a CU where fewer fit), and no more than the same number of turns
+// over the rows needs.
 Grid make_grid(int B, int T, bool by_item, int rows_per_turn, int most) {
     Grid g;
     g.items = by_item ? B : 1;
@@ -383,7 +385,7 @@ template <typename K>
 int resident_blocks(K kernel, int threads) {
     int per_cu = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0) != hipSuccess || per_cu < 1) per_cu = 1;
-    return 256 * (per_cu < 4 ? per_cu : 4);
+    return 256 * (per_cu < 4 ? per_cu : 4);  // (the card's 256 CUs; MAX_PARTS at the most, which sizes the workspace)
 }
 
 bool aligned(const void* p, size_t bytes) { return !((uintptr_t)p & (bytes - 1)); }

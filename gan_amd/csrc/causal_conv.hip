@@ -1,13 +1,15 @@
 // Short causal depthwise convolution along time (+ SiLU) with a carried window, on channels-last activations:
 //   pre[b][t][c] = bias[c] + sum_k w[c][k] x[b][t - (K-1) + k][c],  y = act(pre),  rows before 0 from the window (or zero)
-// forward, backward and the single-token step.  HBM-bound: a few multiply-adds for each element read and written.
+// forward, backward and the single-token step.  Bound by memory where the activations are large, else by vector issue.
 //
 // A thread owns V adjacent channels (one 8- or 16-byte access a row where alignment allows) and a run of rows, the last K of them in registers:
 // slot (K-1 + r) mod K holds the run's row r, so that a turn of K rows moves nothing.  A row is read once by its run and K - 1 rows of every
 // run again by the next one (from cache, mostly); the loads of the next K rows are in flight while K rows are worked on.
 //
 // Measured, bf16, four taps and SiLU: 16 x 2250 x 1024 forward 29 us (147 MB: 5.0 TB/s), backward 60 us (221 MB: 3.7 TB/s, the sums of dw and the
-// activation's slope beside it); 64 x 375 x 512 14.5 and 28.5 us; one row of 64 x 1024 2.7 us, of 256 x 2048 4.6 us.
+// activation's slope beside it); channel slices of wider rows 30 and 61 us; float32 52 and 100 us (5.7 and 4.4 TB/s).  64 x 375 x 512 14.6 and
+// 28.6 us: 2.7 and 2.4 TB/s of memory traffic, the vector units busy 68 and 81 % of the time with 21 and 49 instructions an element; float32 18 and
+// 42 us.  One row of 64 x 1024 2.7 us, of 256 x 2048 4.6 us.
 #include "seq_common.h"
 
 namespace {
@@ -23,8 +25,9 @@ struct Map {
     long runs;       // of all items
 };
 
-// Runs as long as 1024 blocks (four a CU) allow, 16 to 128 rows: the K - 1 rows read twice are then at most a fifth.  (16 x 2250 x 1024 bf16:
-// 29 + 60 us; 33 + 58 with 512 blocks, 31 + 69 with 2048.  64 x 375 x 512: 14.5 + 28.5, 15.2 + 28.2, 14.7 + 29.1.)
+// Runs as long as 1024 blocks (four a CU) allow, 16 to 128 rows: the K - 1 rows read twice are (K - 1) / 16 of them at the most, a fifth with four taps
+// and 44 % with eight.  (16 x 2250 x 1024 bf16: 29 + 60 us; 32 + 57 with 512 blocks, 31 + 69 with 2048.  64 x 375 x 512: 14.6 + 28.6, 15.0 + 28.3,
+// 14.6 + 29.1.)
 Map make_map(int B, int T, int C, int vec) {
     Map m;
     m.pieces = (C + vec - 1) / vec;
@@ -310,7 +313,7 @@ int bwd(const ga_causal_conv_bwd_params& p, hipStream_t s) {
 
 template <typename T, int V, typename P, typename F> int by_taps(const P& p, F f) {
     // Window, gradients and weights of five taps and more for four channels do not fit the registers.  (K = 8: 16 + 40 us at 64 x 375 x 512 bf16, K = 4
-    // 14.5 + 28.5.  Single channels, where widths or bases leave no wider access: K = 4 17.4 + 31.9, at 16 x 2250 x 1024 43 + 84 us against 29 + 60.)
+    // 14.6 + 28.6.  Single channels, where widths or bases leave no wider access: K = 4 17.4 + 31.7, at 16 x 2250 x 1024 43 + 84 us against 29 + 60.)
     switch (p.K) {
         case 1: return f.template go<T, V, 1>(p);
         case 2: return f.template go<T, V, 2>(p);

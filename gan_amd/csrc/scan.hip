@@ -8,12 +8,16 @@
 // Time is cut into chunks where channels and items alone do not fill the card: a first kernel walks every chunk from zero, a small one carries
 // the states from chunk to chunk, the main one then walks each chunk from the state that comes in.
 //
-// Bound by instruction issue: a state and row is a multiply and an exp2 for the decay, a multiply and two multiply-adds (exp2 alone takes the time
-// of two others), and walks through the first kernel (two thirds of it) as well.  At 16 x 2250 x 1024 with 16 states, bf16: forward 270 us
-// (first kernel 115, main 176; 227 MB, 46 us of memory time), with the saved states 275; backward 619 us (first 121, main 522, sums 28; the states
-// walked again, the adjoint, and sums over 64 channels for dB and dC).  12 x 375 x 512: 40 and 66 us; one prompt of 2250 x 512: 32 us.  8 states 187
-// and 405 us; half the items with 32 states 248 and 929 us (a wave's 8 states take turns, the rest waits in LDS, one block a CU); a quarter
-// with 64 states 243 and 831 us.
+// Bound by vector issue.  Counted at 16 x 2250 x 1024 with 16 states, bf16, for a state and row: 7.8 vector instructions forward and 22.6 backward (the
+// states walked again, the adjoint, sums over 64 channels for dB and dC), 5.1 and 5.4 more in the first kernels, all that is done once per row and
+// channel included; an exp2 in each of the four takes the time of two others.  The vector units are busy 92 % of the forward main kernel's time, 83 %
+// of the backward one's (two waves a SIMD: registers), 94 and 93 % of the first kernels'.
+// Times of whole passes, replayed from a graph: at that size forward 269 us (227 MB, 46 us of memory time), 274 with the saved states, backward 616;
+// a process's first passes take up to 8 % more.  Kernel by kernel, which adds up to more: forward maps 6, first 120, carry 6, main 184; backward
+// first 126, carry 6, main 544, sums 28.  12 x 375 x 512: 39 and 66 us; one prompt of 2250 x 512: 32 us.  Float32 at 16 x 2250 x 1024: 281 and 706 us.
+// 8 states 185 and 404 us; half the items with 32 states 247 and 928 us (a wave's 8 states take turns, the rest waits in LDS, one block a CU); a
+// quarter with 64 states 241 and 831 us.  Numbers of states between these pay for the next one: 12 states 266 and 605 us, half the items with 17
+// 242 and 899 us, a quarter with 33 234 and 800 us.
 #include "seq_common.h"
 
 namespace {
@@ -46,8 +50,9 @@ Plan make_plan(int B, int T, int C, int N, int G) {
     q.nCb = q.cbg * G;
     q.tiles = (T + TS - 1) / TS;
     const long blocks = (long)B * q.nCb;
-    // Chunks for four blocks a CU, and for eight where a chunk is still long enough (16 tiles) not to notice its start: the forward pass of
-    // 16 x 2250 x 1024 takes 287 us with eight, 295 with four, 311 with two; 12 x 375 x 512 39 us with four, 44 with eight.
+    // Chunks for four blocks a CU, and for eight where a chunk is still long enough (16 tiles) not to notice its start: 16 x 2250 x 1024, as a
+    // process's first work, takes 291 + 616 us with eight, 295 + 626 with four, 314 + 634 with two; 12 x 375 x 512 38 + 66 us with four, 43 + 73 with
+    // eight.
     long want = (1024 + blocks - 1) / blocks;
     if (q.tiles / want >= 16) want = (2048 + blocks - 1) / blocks;
     if (want > MAX_CHUNKS) want = MAX_CHUNKS;
@@ -129,8 +134,8 @@ __device__ __forceinline__ T at(const void* base, unsigned d) { return *(const T
 
 template <typename T> struct alignas(4 * sizeof(T)) Quad { T v[4]; };
 
-// The four elements of a tile that a lane prepares and finishes.  (16 x 2250 x 1024 x 16 bf16: 270 + 619 us; one channel at a time 276 + 725.)  VEC: four adjacent channels of one row, one access for all four rows of a wave;
-// otherwise (alignment, odd widths) one channel of each of the four rows.
+// The four elements of a tile that a lane prepares and finishes.  VEC: four adjacent channels of one row, one access for all four rows of a wave;
+// otherwise (alignment, odd widths) one channel of each of the four rows.  (16 x 2250 x 1024 x 16 bf16: 269 + 616 us; one channel at a time 275 + 726.)
 template <bool VEC>
 struct Elems {
     int lane, w, g, first, Cg;  // first: the block's first channel in its group
@@ -567,7 +572,9 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void scan_bwd_kernel(BwdArgs 
     const ga_scan_bwd_params& p = a.p;
     const Plan& q = a.q;
     constexpr int NB = NS < 4 ? NS : 4, SB = NS / NB, U = 2;
-    constexpr bool AHEAD = SB == 1 && VEC && sizeof(T) == 2;  // the next tile's rows on their way (float32 rows, or ones of single channels, spill)
+    // the next tile's rows on their way (float32 rows, or ones of single channels, spill: they are loaded where they are used, and the pass of
+    // 16 x 2250 x 1024 x 16 takes 706 and 726 us in place of 616)
+    constexpr bool AHEAD = SB == 1 && VEC && sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) float2 sd[TS][64];     // step, step * u
     __shared__ __attribute__((aligned(16))) float sg[TS][64];      // dy * gate
     __shared__ __attribute__((aligned(16))) float sy[4][TS][64];   // <C, h> over a wave's states
@@ -899,7 +906,7 @@ __global__ __launch_bounds__(1024) void scan_dparams_kernel(const float* __restr
 }
 
 // One token: a thread holds four states of a channel, 1 << shift threads a channel, a block channels of one item (nb blocks an item); the state is
-// read and written once, and everything else is small: 256 x 1024 x 16 states, bf16, 7.8 us (35.7 MB: 4.6 TB/s), 17.5 with single elements of
+// read and written once, and everything else is small: 256 x 1024 x 16 states, bf16, 7.8 us (35.7 MB: 4.6 TB/s), 17.3 with single elements of
 // state, A, B and C (odd N or unaligned bases); 256 x 1024 x 64 28 us; one item of 512 x 16 2.5 us.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(ga_scan_step_params p, int shift, unsigned nb) {
@@ -976,7 +983,7 @@ int grid_for(size_t n) {
 int launch_carry(const float* A, const float* first, float* ends, const float* ends_step, const Plan& q, int B, int C, int N, int dir, hipStream_t s) {
     const size_t states = (size_t)B * N * C;  // (2^23 at the most: sequences are cut where there are fewer than 2048 blocks of 64 channels)
     static_assert(MAX_CHUNKS <= 16 * 16, "runs of the carry kernel");
-    // (8 chunks at 16 x 2250 x 1024: 5.6 us, 8.3 with loads for 32; 32 chunks at 4 x 2250 x 512: the whole forward pass 62 us, 67 with 16 runs)
+    // (the whole forward pass, 8 chunks at 16 x 2250 x 1024: 291 us, 296 with loads for 32; 32 chunks at 4 x 2250 x 512: 63 us, 66 with 16 runs)
     if (q.chunks <= 8) scan_carry_kernel<1, 8><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
     else if (q.chunks <= 32) scan_carry_kernel<1, 32><<<(unsigned)((states + 255) / 256), 256, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);
     else scan_carry_kernel<16, 16><<<(unsigned)((states + 63) / 64), 1024, 0, s>>>(A, first, ends, ends_step, q, B, C, N, dir);

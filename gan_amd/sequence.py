@@ -13,8 +13,8 @@ what is returned in bfloat16 is rounded once.  An activation may be a channel sl
 anything else that is not packed is copied.  Calls enqueue on the current stream of the tensors' device and keep nothing between calls, so they
 may be captured into graphs and run on several streams at once; results do not depend on timing (no atomics).  Gradients are of first order and in
 reverse mode (a tensor with a forward-mode tangent is refused, NotImplementedError); a backward pass is captured with torch.autograd.grad, or
-with leaves of which no eager graph is alive (a leaf's accumulation belongs to the stream that first used it).  delta = -inf (or the type's
-lowest value) is a step of zero: the row leaves the states as they are.
+with leaves of which no eager graph is alive (a leaf's accumulation belongs to the stream that first used it).  Under softplus delta = -inf
+(or the type's lowest value) is a step of zero: the row leaves the states as they are.
 Sizes and types are checked here (ValueError / TypeError); like every operator of this package these run on the GPU only.
 """
 from __future__ import annotations
@@ -367,7 +367,8 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, Bm: Tensor, Cm: Tensor, 
     single row's factor exp(step * A) has to be inside float32, the product over many rows need not), D, delta_bias [C], state [B, C, N] (the
     states before row 0, zero without it): float32.  `lengths` as in causal_conv: rows behind an item's end leave its state alone, give y = 0 and
     get no gradient.  With `return_state` also the states at each item's end, float32 [B, C, N].
-    Differentiable in every tensor but `lengths`; the backward pass keeps the state at every 16th row (C * N / 16 floats a row)."""
+    Differentiable in every tensor but `lengths`; for the backward pass C * P / 16 + 2 * G * P floats a row are kept (the state at every 16th row, B
+    and C), with P = 8, 16, 32 or 64 for N up to that."""
     if u.dim() != 3 or 0 in u.shape:
         raise ValueError(f"u: expected a non-empty [B, T, C], got {tuple(u.shape)}")
     Bm, Cm = _scan_checks(u, delta, A, Bm, Cm, D, z, delta_bias, state)
